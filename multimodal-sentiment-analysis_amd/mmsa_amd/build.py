@@ -12,7 +12,10 @@ LIB_PATH = os.path.join(PKG_DIR, "libmmsa_hip.so")
 OBJ_DIR = os.path.join(CSRC, "build")
 SOURCES = ("frontend.hip", "denoise.hip", "conv.hip", "wgrad.hip", "audio_ew.hip", "text.hip", "dense.hip", "head.hip", "optim.hip")
 FLAGS = ["--offload-arch=gfx950", "-O3", "-fPIC", "-std=c++17", "-fvisibility=hidden", "-Wall",
-         "-Wno-unused-function"]
+         "-Wno-unused-function",
+         # no packed fp32 arithmetic: some of its forms have given wrong results on this hardware now and then
+         # (the host pass does not know the feature and says so)
+         "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 
 
 def _hipcc() -> str:
