@@ -96,5 +96,5 @@ def query(name: str, *args):
     fn = getattr(load(), name)
     rc = fn(*args)
     if rc < 0:
-        raise MmsaError(f"{name} rejected its arguments (status {rc})")
+        raise MmsaError(f"{name} rejected its arguments (status {rc}{', limit exceeded' if rc == -3 else ''})")
     return rc

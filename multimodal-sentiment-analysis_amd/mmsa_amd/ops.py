@@ -220,6 +220,66 @@ def denoise(wave: torch.Tensor, filt, tables, out: Optional[torch.Tensor] = None
     return out
 
 
+# ------------------------------------------------------------------------- group normalisation with an activation
+ACTIVATIONS = {"none": 0, "relu": 1, "silu": 2, "gelu": 3}
+DTYPE_CODES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+
+
+def _group_norm_args(x, gamma, beta, groups, act):
+    if x.dim() != 3:
+        raise ValueError("group_norm_act: x must be [B, positions, channels]")
+    if x.dtype not in DTYPE_CODES:
+        raise TypeError(f"group_norm_act: float32, bfloat16 or float16 maps, got {x.dtype}")
+    if act not in ACTIVATIONS:
+        raise ValueError(f"group_norm_act: activation {act!r} is none of {', '.join(ACTIVATIONS)}")
+    B, P, C = x.shape
+    if groups < 1 or C < 1 or C % groups:
+        raise ValueError(f"group_norm_act: {C} channels do not divide into {groups} groups")
+    for t, name in ((gamma, "weight"), (beta, "bias")):
+        if t is not None and tuple(t.shape) != (C,):
+            raise ValueError(f"group_norm_act: {name} must be [{C}]")
+    return B, P, C
+
+
+def _group_norm_scratch(x, groups):
+    B, P, C = x.shape
+    n = _lib.query("mmsa_group_norm_act_scratch_bytes", B, P, C, groups, DTYPE_CODES[x.dtype])
+    return torch.empty(((n + 7) // 8,), dtype=torch.float64, device=x.device)
+
+
+def group_norm_act_fwd(x, gamma, beta, y, stats, groups: int, eps: float = 1e-5, act: str = "none"):
+    """y = act(group_norm(x) * gamma + beta) over x [B, P, C]; stats [B, groups, 2] float64 <- mean, 1/sqrt(var + eps).
+    gamma / beta [C] float32, or None for 1 / 0."""
+    B, P, C = _group_norm_args(x, gamma, beta, groups, act)
+    if y.shape != x.shape or tuple(stats.shape) != (B, groups, 2):
+        raise ValueError("group_norm_act_fwd: y like x, stats [B, groups, 2]")
+    if x.numel() == 0:
+        return y
+    _lib.call("mmsa_group_norm_act_fwd", _chk(x, x.dtype, "x"), _opt(gamma, F32, "weight"), _opt(beta, F32, "bias"),
+              _chk(y, x.dtype, "y"), _chk(stats, torch.float64, "stats"), _group_norm_scratch(x, groups).data_ptr(),
+              B, P, C, groups, eps, ACTIVATIONS[act], DTYPE_CODES[x.dtype], _stream())
+    return y
+
+
+def group_norm_act_bwd(dy, x, gamma, beta, stats, dx, dgamma, dbeta, groups: int, act: str = "none"):
+    """Gradients of :func:`group_norm_act_fwd`; dx, dgamma, dbeta may each be None (not wanted)."""
+    B, P, C = _group_norm_args(x, gamma, beta, groups, act)
+    if dy.shape != x.shape or (dx is not None and dx.shape != x.shape) or tuple(stats.shape) != (B, groups, 2):
+        raise ValueError("group_norm_act_bwd: dy and dx like x, stats [B, groups, 2]")
+    for t in (dgamma, dbeta):
+        if t is not None and tuple(t.shape) != (C,):
+            raise ValueError("group_norm_act_bwd: dgamma and dbeta [C]")
+    if x.numel() == 0:
+        for t in (dgamma, dbeta):
+            if t is not None:
+                t.zero_()
+        return
+    _lib.call("mmsa_group_norm_act_bwd", _chk(dy, x.dtype, "dy"), _chk(x, x.dtype, "x"), _opt(gamma, F32, "weight"),
+              _opt(beta, F32, "bias"), _chk(stats, torch.float64, "stats"), _opt(dx, x.dtype, "dx"),
+              _opt(dgamma, F32, "dgamma"), _opt(dbeta, F32, "dbeta"), _group_norm_scratch(x, groups).data_ptr(),
+              B, P, C, groups, ACTIVATIONS[act], DTYPE_CODES[x.dtype], _stream())
+
+
 # ---------------------------------------------------------------------------------------------- convolution
 def pack_weights(w: torch.Tensor, fwd: Optional[torch.Tensor], dgrad: Optional[torch.Tensor]):
     cout, cin = w.shape[0], w.shape[1]

@@ -112,3 +112,10 @@ _reg("fusion_mix_bwd", "(Tensor dfused, Tensor P, Tensor wts, Tensor(a!) dP, Ten
 _reg("softmax_ce", "(Tensor logits, Tensor? labels, Tensor(a!) probs, Tensor(b!)? loss, Tensor(c!)? dlogits) -> ()",
      ops.softmax_ce)
 _reg("dropout", "(Tensor x, Tensor(a!) y, float drop_p, int seed, Tensor? step=None) -> ()", ops.dropout)
+
+# ---- group normalisation with an activation, channels last ----------------------------------------------------------
+_reg("group_norm_act_fwd", "(Tensor x, Tensor? gamma, Tensor? beta, Tensor(a!) y, Tensor(b!) stats, int groups, "
+                           "float eps=1e-05, str act='none') -> ()", ops.group_norm_act_fwd)
+_reg("group_norm_act_bwd", "(Tensor dy, Tensor x, Tensor? gamma, Tensor? beta, Tensor stats, Tensor(a!)? dx, "
+                           "Tensor(b!)? dgamma, Tensor(c!)? dbeta, int groups, str act='none') -> ()",
+     ops.group_norm_act_bwd)
