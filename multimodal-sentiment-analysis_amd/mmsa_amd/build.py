@@ -11,7 +11,7 @@ CSRC = os.path.join(os.path.dirname(PKG_DIR), "csrc")
 LIB_PATH = os.path.join(PKG_DIR, "libmmsa_hip.so")
 OBJ_DIR = os.path.join(CSRC, "build")
 SOURCES = ("frontend.hip", "denoise.hip", "conv.hip", "wgrad.hip", "audio_ew.hip", "text.hip", "dense.hip", "head.hip", "optim.hip",
-           "norm.hip")
+           "norm.hip", "muon.hip")
 FLAGS = ["--offload-arch=gfx950", "-O3", "-fPIC", "-std=c++17", "-fvisibility=hidden", "-Wall",
          "-Wno-unused-function",
          # no packed fp32 arithmetic: some of its forms have given wrong results on this hardware now and then

@@ -1096,3 +1096,64 @@ def scale_by_state(g, state, idx):
 
 def scalar_axpy(dst, a, b, alpha):
     _lib.call("mmsa_scalar_axpy", _chk(dst), _chk(a), _chk(b), float(alpha), _stream())
+
+
+# ------------------------------------------------------------------------------------------- orthogonalised updates
+def _matrices(ts, dtype, name):
+    for t in ts:
+        if t.dim() != 2 or t.numel() == 0:
+            raise ValueError(f"{name}: non-empty matrices [rows, cols], got {tuple(t.shape)}")
+    if len({t.device for t in ts}) > 1:
+        raise ValueError(f"{name}: the matrices of one call live on one device")
+    return _parr([_chk(t, dtype, name) for t in ts])
+
+
+def _ns_args(steps, eps):
+    if not 1 <= int(steps) <= 16 or int(steps) != steps:
+        raise ValueError("steps must be a whole number from 1 to 16")
+    if not float(eps) > 0.0:
+        raise ValueError("eps must be positive")
+
+
+def _ns_scratch(rows, cols, n, device):
+    return torch.empty((_lib.query("mmsa_orthogonalize_scratch_bytes", rows, cols, n),), dtype=torch.uint8, device=device)
+
+
+def orthogonalize(srcs, dsts, steps: int = 5, eps: float = 1e-7):
+    """dsts[i] <- the Newton-Schulz orthogonalisation of srcs[i] ([rows, cols], one dtype for all), in shared launches."""
+    _ns_args(steps, eps)
+    if len(srcs) != len(dsts) or any(a.shape != b.shape for a, b in zip(srcs, dsts)):
+        raise ValueError("orthogonalize: one destination like every source")
+    if not srcs:
+        return
+    dtype = srcs[0].dtype
+    if dtype not in DTYPE_CODES:
+        raise TypeError(f"orthogonalize: float32, bfloat16 or float16 matrices, got {dtype}")
+    n = len(srcs)
+    src, dst = _matrices(srcs, dtype, "orthogonalize"), _matrices(dsts, dtype, "orthogonalize")
+    if dsts[0].device != srcs[0].device:
+        raise ValueError("orthogonalize: the matrices of one call live on one device")
+    rows, cols = _iarr([t.shape[0] for t in srcs]), _iarr([t.shape[1] for t in srcs])
+    stream = _stream()
+    _lib.call("mmsa_orthogonalize", src, dst, rows, cols, n, DTYPE_CODES[dtype], int(steps), eps,
+              _ns_scratch(rows, cols, n, srcs[0].device).data_ptr(), stream)
+
+
+def muon_step(params, grads, momenta, lr, weight_decay, momentum, nesterov=True, steps: int = 5, eps: float = 1e-7):
+    """One Muon step over fp32 matrices [rows, cols]; params and momenta are updated in place."""
+    _ns_args(steps, eps)
+    if not len(params) == len(grads) == len(momenta) or any(p.shape != g.shape or p.shape != m.shape
+                                                            for p, g, m in zip(params, grads, momenta)):
+        raise ValueError("muon_step: one gradient and one momentum buffer like every parameter")
+    if not params:
+        return
+    n = len(params)
+    ptrs = [_matrices(ts, F32, name) for ts, name in ((params, "params"), (grads, "grads"), (momenta, "momenta"))]
+    if not params[0].device == grads[0].device == momenta[0].device:
+        raise ValueError("muon_step: the matrices of one call live on one device")
+    if len(set(ptrs[0]) | set(ptrs[2])) != 2 * n or set(ptrs[1]) & (set(ptrs[0]) | set(ptrs[2])):
+        raise ValueError("muon_step: a parameter or momentum buffer is listed twice")
+    rows, cols = _iarr([t.shape[0] for t in params]), _iarr([t.shape[1] for t in params])
+    stream = _stream()
+    _lib.call("mmsa_muon_step", *ptrs, rows, cols, n, float(lr), float(weight_decay), float(momentum), int(nesterov),
+              int(steps), eps, _ns_scratch(rows, cols, n, params[0].device).data_ptr(), stream)
