@@ -15,8 +15,8 @@
 // A matrix whose norm is below eps enters with entries far below 1: its X is held at a larger scale 2^(14 + k), k from
 // the norm (the polynomial grows it by at most a per step, so k shrinks from step to step by the same bound).
 //
-// Layout.  A padded matrix [rows][K] of pairs is stored as [row][K / 32][hi 32 | lo 32] fp16: 32 values of a row are
-// one 128-byte line holding both halves, which is what a K step of the products reads.  All products are row times row
+// Layout.  A padded matrix [rows][K] of pairs is stored as [row][K / 16][hi 16 | lo 16] fp16: 16 values of a row, what
+// one matrix instruction takes, are 64 bytes holding both halves.  All products are row times row
 // (both operands K-contiguous): X X^T, T T (T is symmetric), and B X = B (X^T)^T, for which X^T is kept beside X.
 // Padding rows and columns hold zeros and stay zero.
 #include "mmsa_common.h"
@@ -65,16 +65,17 @@ static_assert(sizeof(Group) < 4096 - 256, "kernel arguments are limited to 4 KiB
 
 // scratch of one matrix: X [mp][np], X^T [np][mp] twice (read and written in turn), T and B [mp][mp], k per step, the
 // partial tiles of a split product
-__host__ __device__ inline long xbytes(const Mat& q) { return 4l * q.mp * q.np; }
-__host__ __device__ inline long sbytes(const Mat& q) { return 4l * q.mp * q.mp; }
+__host__ __device__ inline long row_bytes(long K) { return 4 * K; }
+__host__ __device__ inline long xbytes(const Mat& q) { return q.mp * row_bytes(q.np); }
+__host__ __device__ inline long tbytes(const Mat& q) { return q.np * row_bytes(q.mp); }
+__host__ __device__ inline long sbytes(const Mat& q) { return q.mp * row_bytes(q.mp); }
+__host__ __device__ inline long mat_bytes(const Mat& q) { return xbytes(q) + 2 * tbytes(q) + 2 * sbytes(q) + 128; }
 __device__ __forceinline__ char* ws_x(const Mat& q) { return q.ws; }
-__device__ __forceinline__ char* ws_xt(const Mat& q, int which) { return q.ws + (1 + which) * xbytes(q); }
-__device__ __forceinline__ char* ws_t(const Mat& q) { return q.ws + 3 * xbytes(q); }
-__device__ __forceinline__ char* ws_b(const Mat& q) { return q.ws + 3 * xbytes(q) + sbytes(q); }
-__device__ __forceinline__ int* ws_k(const Mat& q) { return reinterpret_cast<int*>(q.ws + 3 * xbytes(q) + 2 * sbytes(q)); }
-__device__ __forceinline__ float* ws_part(const Mat& q) {
-  return reinterpret_cast<float*>(q.ws + 3 * xbytes(q) + 2 * sbytes(q) + 128);
-}
+__device__ __forceinline__ char* ws_xt(const Mat& q, int which) { return q.ws + xbytes(q) + which * tbytes(q); }
+__device__ __forceinline__ char* ws_t(const Mat& q) { return q.ws + xbytes(q) + 2 * tbytes(q); }
+__device__ __forceinline__ char* ws_b(const Mat& q) { return q.ws + xbytes(q) + 2 * tbytes(q) + sbytes(q); }
+__device__ __forceinline__ int* ws_k(const Mat& q) { return reinterpret_cast<int*>(q.ws + mat_bytes(q) - 128); }
+__device__ __forceinline__ float* ws_part(const Mat& q) { return reinterpret_cast<float*>(q.ws + mat_bytes(q)); }
 
 // which matrix a block works on: the last one whose first block is not behind it (all lanes of a wave call it)
 __device__ __forceinline__ int find_mat(const int* first, int count, int block) {
@@ -85,10 +86,17 @@ __device__ __forceinline__ int find_mat(const int* first, int count, int block) 
 }
 
 // ---- element types
+// four values at any alignment of one value (this target's global accesses allow it)
+typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));
+typedef unsigned u32x2u __attribute__((ext_vector_type(2), aligned(2)));
 template <typename T> struct El;
 template <> struct El<float> {
   static __device__ __forceinline__ float get(const void* p, long i) { return static_cast<const float*>(p)[i]; }
   static __device__ __forceinline__ void put(void* p, long i, float v) { static_cast<float*>(p)[i] = v; }
+  static __device__ __forceinline__ void put4(void* p, long i, f32x4 v) {
+    f32x4u u = {v[0], v[1], v[2], v[3]};
+    *reinterpret_cast<f32x4u*>(static_cast<float*>(p) + i) = u;
+  }
 };
 template <> struct El<__hip_bfloat16> {
   static __device__ __forceinline__ float get(const void* p, long i) {
@@ -97,12 +105,24 @@ template <> struct El<__hip_bfloat16> {
   static __device__ __forceinline__ void put(void* p, long i, float v) {
     static_cast<__hip_bfloat16*>(p)[i] = __float2bfloat16(v);
   }
+  static __device__ __forceinline__ void put4(void* p, long i, f32x4 v) {
+    __hip_bfloat16 h[4] = {__float2bfloat16(v[0]), __float2bfloat16(v[1]), __float2bfloat16(v[2]), __float2bfloat16(v[3])};
+    u32x2u u;
+    __builtin_memcpy(&u, h, 8);
+    *reinterpret_cast<u32x2u*>(static_cast<__hip_bfloat16*>(p) + i) = u;
+  }
 };
 template <> struct El<_Float16> {
   static __device__ __forceinline__ float get(const void* p, long i) {
     return (float)static_cast<const _Float16*>(p)[i];
   }
   static __device__ __forceinline__ void put(void* p, long i, float v) { static_cast<_Float16*>(p)[i] = (_Float16)v; }
+  static __device__ __forceinline__ void put4(void* p, long i, f32x4 v) {
+    _Float16 h[4] = {(_Float16)v[0], (_Float16)v[1], (_Float16)v[2], (_Float16)v[3]};
+    u32x2u u;
+    __builtin_memcpy(&u, h, 8);
+    *reinterpret_cast<u32x2u*>(static_cast<_Float16*>(p) + i) = u;
+  }
 };
 
 __device__ __forceinline__ float direction(float g, float mom, float mu, int nesterov) {
@@ -140,9 +160,9 @@ __global__ __launch_bounds__(256) void momentum_sumsq_kernel(const Group gr, flo
 
 __device__ __forceinline__ void put_pair(char* base, long row, long col, long K, float v) {
   const _Float16 hi = (_Float16)v;
-  _Float16* p = reinterpret_cast<_Float16*>(base) + row * 2 * K + (col >> 5) * 64 + (col & 31);
+  _Float16* p = reinterpret_cast<_Float16*>(base + row * row_bytes(K)) + (col >> 4) * 32 + (col & 15);
   p[0] = hi;
-  p[32] = (_Float16)(v - (float)hi);
+  p[16] = (_Float16)(v - (float)hi);
 }
 
 // how far X's scale exceeds 2^NS_SCALE for a bound r on its norm
@@ -229,190 +249,352 @@ __device__ __forceinline__ float diagonal() {
   return ldexpf(MODE == TO_T ? NS_SHIFT : NS_REST, NS_SCALE);
 }
 
-// D = P Q^T over K for one BT x BT tile, four waves as 2 x 2, both operands staged through LDS in K steps of 32 values
-// (128-byte rows, their 16-byte units XORed with the row so that the fragment reads spread over the banks).
+// The order in which a matrix's tiles are given to its blocks: consecutive blocks go to the eight XCDs in turn, each
+// with an L2 of its own, so every XCD gets one consecutive run of tiles (whose operand rows it shares).
+__device__ __forceinline__ int xcd_order(int l, int n) {
+  const int per = n >> 3;
+  return l < per << 3 ? (l & 7) * per + (l >> 3) : l;
+}
+
+// Shape of a product block: BT x BT outputs, four waves as 2 x 2, each with W x W tiles of 32 x 32.
+template <int BT>
+struct Tile {
+  static constexpr int W = BT / 64;
+  static constexpr int G = BT == 256 ? 1 : 2;         // groups of 16 values of K in a step
+  static constexpr int ROW = 64 * G;                    // bytes of an operand row in one LDS buffer
+  static constexpr int OPER = BT * ROW;
+  static constexpr int RING = 4;                        // LDS buffers
+  static constexpr int LOADS = BT * G / 32;             // a thread's loads per step
+  static constexpr int PASSES = BT == 256 ? 2 : 1;      // rounds in which the results leave through LDS
+  static constexpr int OUTROW = BT * 4 + 16;            // an output row of pairs in LDS, padded against bank conflicts
+  static constexpr int LDS = RING * 2 * OPER > BT / PASSES * OUTROW ? RING * 2 * OPER : BT / PASSES * OUTROW;
+};
+
+// waits until at most N of this wave's global loads are on their way (they return in order) and its LDS reads are done,
+// then for the other waves
+template <int N>
+__device__ __forceinline__ void wait_loads_and_meet() {
+  static_assert(N >= 0 && N < 64, "six bits");
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_waitcnt((N & 15) | 7 << 4 | (N >> 4) << 14);
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
+
+// acc += P Q^T over nk32 * 32 values.  Each wave runs ahead of itself: a ring of four LDS buffers, loads straight into LDS
+// issued three steps ahead and waited for by count, and the fragments of the next step read while the matrix
+// instructions of this one run, one load or read between two of them.  The 16-byte units of a row are XORed with bits of
+// the row, which makes the fragment reads free of bank conflicts: 16 lanes of one read cover the 16 units of 256 bytes.
+template <int BT>
+struct Fragments {
+  f16x8 ph[Tile<BT>::G][Tile<BT>::W], pl[Tile<BT>::G][Tile<BT>::W];
+  f16x8 qh[Tile<BT>::G][Tile<BT>::W], ql[Tile<BT>::G][Tile<BT>::W];
+};
+
+template <int BT>
+__device__ __forceinline__ void multiply(f32x16 (&acc)[Tile<BT>::W][Tile<BT>::W], char* lds, const char* P,
+                                         const char* Q, long pitch, int nk32) {
+  typedef Tile<BT> S;
+  constexpr int W = S::W, G = S::G, ROW = S::ROW, OPER = S::OPER, LOADS = S::LOADS;
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+  const int nk = nk32 * 2 / G;
+  // a wave's load fills 16 / G rows
+  const int lrow = lane / (4 * G), lu = lane % (4 * G);
+  const int lunit = lu ^ (G == 1 ? (lrow >> 2) & 3 : ((w & 1) * 4 + (lrow >> 1)) & 7);
+  const char* ps = P + (w * (16 / G) + lrow) * pitch + lunit * 16;
+  const char* qs = Q + (w * (16 / G) + lrow) * pitch + lunit * 16;
+  auto stage = [&](int k) {
+    char* to = lds + (k & 3) * 2 * OPER + w * 1024;
+#pragma unroll
+    for (int j = 0; j < LOADS / 2; ++j) {
+      load_lds16(ps + j * (64 / G) * pitch + (long)k * ROW, to + j * 4096);
+      load_lds16(qs + j * (64 / G) * pitch + (long)k * ROW, to + OPER + j * 4096);
+    }
+  };
+  const int fr = lane & 31, half = lane >> 5, swz = G == 1 ? (fr >> 2) & 3 : (fr >> 1) & 7;
+  const int prow = ((w >> 1) * W * 32 + fr) * ROW, qrow = OPER + ((w & 1) * W * 32 + fr) * ROW;
+  auto fetch = [&](Fragments<BT>& f, int k) {
+    const char* l0 = lds + (k & 3) * 2 * OPER;
+#pragma unroll
+    for (int s = 0; s < G; ++s) {
+      const int uh = ((s * 4 + half) ^ swz) * 16, ul = ((s * 4 + 2 + half) ^ swz) * 16;
+#pragma unroll
+      for (int x = 0; x < W; ++x) {
+        f.qh[s][x] = *reinterpret_cast<const f16x8*>(l0 + qrow + x * 32 * ROW + uh);
+        f.ql[s][x] = *reinterpret_cast<const f16x8*>(l0 + qrow + x * 32 * ROW + ul);
+        f.ph[s][x] = *reinterpret_cast<const f16x8*>(l0 + prow + x * 32 * ROW + uh);
+        f.pl[s][x] = *reinterpret_cast<const f16x8*>(l0 + prow + x * 32 * ROW + ul);
+      }
+    }
+  };
+  auto compute = [&](const Fragments<BT>& f) {
+#pragma unroll
+    for (int s = 0; s < G; ++s)
+#pragma unroll
+      for (int x = 0; x < W; ++x) {
+#pragma unroll
+        for (int y = 0; y < W; ++y)
+          acc[x][y] = __builtin_amdgcn_mfma_f32_32x32x16_f16(f.pl[s][x], f.qh[s][y], acc[x][y], 0, 0, 0);
+#pragma unroll
+        for (int y = 0; y < W; ++y)
+          acc[x][y] = __builtin_amdgcn_mfma_f32_32x32x16_f16(f.ph[s][x], f.ql[s][y], acc[x][y], 0, 0, 0);
+#pragma unroll
+        for (int y = 0; y < W; ++y)
+          acc[x][y] = __builtin_amdgcn_mfma_f32_32x32x16_f16(f.ph[s][x], f.qh[s][y], acc[x][y], 0, 0, 0);
+      }
+  };
+  // Step k: step k + 1 has arrived for all waves, so its fragments can be read; the buffer of step k + 3 held step
+  // k - 1, whose fragments every wave had before it came here.  The reads and loads are spread over the matrix
+  // instructions, none of which depends on them.
+  auto step = [&](const Fragments<BT>& now, Fragments<BT>& next, int k) {
+    wait_loads_and_meet<LOADS>();
+    stage(k + 3);
+    fetch(next, k + 1);
+    compute(now);
+#pragma unroll
+    for (int i = 0; i < LOADS; ++i) {
+      __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);            // matrix
+      __builtin_amdgcn_sched_group_barrier(0x020, 1, 0);            // global load
+    }
+#pragma unroll
+    for (int i = 0; i < 4 * W * G; ++i) {
+      __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);            // matrix
+      __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);            // LDS read
+    }
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  // nk is even
+  Fragments<BT> a, b;
+  stage(0);
+  stage(1);
+  if (nk == 2) {
+    wait_loads_and_meet<0>();
+    fetch(a, 0);
+    fetch(b, 1);
+    compute(a);
+    compute(b);
+    return;
+  }
+  stage(2);
+  wait_loads_and_meet<2 * LOADS>();
+  fetch(a, 0);
+  int k = 0;
+  for (; k + 4 < nk; k += 2) {
+    step(a, b, k);
+    step(b, a, k + 1);
+  }
+  step(a, b, k);
+  wait_loads_and_meet<0>();
+  fetch(a, k + 2);
+  compute(b);
+  __builtin_amdgcn_sched_barrier(0);
+  fetch(b, k + 3);
+  compute(a);
+  __builtin_amdgcn_sched_barrier(0);
+  compute(b);
+}
+
+// D = P Q^T for one BT x BT tile of one matrix.
 // T and B are symmetric: only tiles on and below the diagonal are computed, the others are written as their mirror
-// image.  Where a phase has few tiles and a long K, `kper` steps of K go to one block each and the partial results
-// meet in join_kernel.
+// image.  Where a phase has few tiles and a long K, a share of the K steps goes to one block each and the partial
+// results meet in join_kernel.
 template <typename T, int BT, int MODE>
-__global__ __launch_bounds__(256) void product_kernel(const Group* __restrict__ grp, int step, int which, float decay,
-                                                      float rate) {
-  constexpr int WT = BT / 64;                 // 32 x 32 tiles a wave has per direction
-  constexpr int OPER = BT * 128;              // bytes of one operand's stage
-  constexpr int OUTROW = BT * 4 + 16;         // an output row of pairs in LDS, padded against bank conflicts
-  __shared__ __attribute__((aligned(128))) char lds[4 * OPER > BT * OUTROW ? 4 * OPER : BT * OUTROW];
+__global__ __launch_bounds__(256, BT == 256 || Tile<BT>::LDS > 81920 ? 1 : 2) void product_kernel(const Group* __restrict__ grp, int step,
+                                                                         int which, float decay, float rate) {
+  typedef Tile<BT> S;
+  constexpr int W = S::W;
+  __shared__ __attribute__((aligned(128))) char lds[S::LDS];
   const Group& gr = *grp;
   constexpr int PHASE = MODE < TO_X ? MODE : TO_X;
   const int mi = find_mat(gr.first[PH_PRODUCT + PHASE], gr.count, blockIdx.x);
   const Mat& q = gr.mat[mi];
-  int b = blockIdx.x - gr.first[PH_PRODUCT + PHASE][mi];
+  const int b = blockIdx.x - gr.first[PH_PRODUCT + PHASE][mi];
   const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
   const int K = MODE == TO_T ? q.np : q.mp;
   int ti, tj, k_lo = 0, nk = K / 32, part = 0, nsplit = 1, tile = 0;
   if (MODE <= TO_B) {
+    const int nt = q.mp / BT;
     nsplit = q.nsplit[PHASE];
-    tile = b / nsplit;
-    part = b % nsplit;
+    const int l = xcd_order(b, nt * (nt + 1) / 2 * nsplit);
+    tile = l / nsplit;
+    part = l % nsplit;
     lower_tile(tile, ti, tj);
-    const int kper = (nk + nsplit - 1) / nsplit;
+    const int kper = ((nk >> 1) + nsplit - 1) / nsplit * 2;      // an even number of steps
     k_lo = part * kper;
     nk = nk - k_lo < kper ? nk - k_lo : kper;
   } else {
-    const int nt = q.np / BT;
-    ti = b / nt;
-    tj = b % nt;
+    // bands of eight tile rows, column by column
+    const int mt = q.mp / BT, nt = q.np / BT;
+    const int l = xcd_order(b, mt * nt);
+    const int band = l / (8 * nt), rows = mt - band * 8 < 8 ? mt - band * 8 : 8, r = l - band * 8 * nt;
+    ti = band * 8 + r % rows;
+    tj = r / rows;
   }
   const char* P = MODE == TO_T ? ws_x(q) : MODE == TO_B ? ws_t(q) : ws_b(q);
   const char* Q = MODE == TO_T ? ws_x(q) : MODE == TO_B ? ws_t(q) : ws_xt(q, which);
-  const long pitch = 4l * K;
-  // staging: a wave's load fills eight rows of 128 bytes
-  const int lrow = lane >> 3, lunit = (lane & 7) ^ lrow;
-  const char* ps = P + ((long)ti * BT + w * 8 + lrow) * pitch + lunit * 16 + k_lo * 128l;
-  const char* qs = Q + ((long)tj * BT + w * 8 + lrow) * pitch + lunit * 16 + k_lo * 128l;
-  auto stage = [&](int buf, int kc) {
+  const long pitch = row_bytes(K);
+  f32x16 acc[W][W];
 #pragma unroll
-    for (int j = 0; j < BT / 32; ++j) {
-      load_lds16(ps + j * 32 * pitch + (long)kc * 128, lds + (buf * 2 + 0) * OPER + (j * 32 + w * 8) * 128);
-      load_lds16(qs + j * 32 * pitch + (long)kc * 128, lds + (buf * 2 + 1) * OPER + (j * 32 + w * 8) * 128);
-    }
-  };
-  f32x16 acc[WT][WT];
+  for (int x = 0; x < W; ++x)
 #pragma unroll
-  for (int x = 0; x < WT; ++x)
-#pragma unroll
-    for (int y = 0; y < WT; ++y)
+    for (int y = 0; y < W; ++y)
 #pragma unroll
       for (int e = 0; e < 16; ++e) acc[x][y][e] = 0.f;
-  const int wi = w >> 1, wj = w & 1;
-  const int fr = lane & 31, half = lane >> 5;
-  if (nk > 0) stage(0, 0);
-  for (int kc = 0; kc < nk; ++kc) {
-    __syncthreads();
-    if (kc + 1 < nk) stage((kc + 1) & 1, kc + 1);
-    const char* lp = lds + (kc & 1) * 2 * OPER;
-    const char* lq = lp + OPER;
-#pragma unroll
-    for (int s = 0; s < 2; ++s) {
-      f16x8 ph[WT], pl[WT], qh[WT], ql[WT];
-#pragma unroll
-      for (int x = 0; x < WT; ++x) {
-        const int rp = wi * (BT / 2) + x * 32 + fr, rq = wj * (BT / 2) + x * 32 + fr;
-        const int u = s * 2 + half;
-        ph[x] = *reinterpret_cast<const f16x8*>(lp + rp * 128 + ((u ^ (rp & 7)) * 16));
-        pl[x] = *reinterpret_cast<const f16x8*>(lp + rp * 128 + (((u + 4) ^ (rp & 7)) * 16));
-        qh[x] = *reinterpret_cast<const f16x8*>(lq + rq * 128 + ((u ^ (rq & 7)) * 16));
-        ql[x] = *reinterpret_cast<const f16x8*>(lq + rq * 128 + (((u + 4) ^ (rq & 7)) * 16));
-      }
-#pragma unroll
-      for (int x = 0; x < WT; ++x)
-#pragma unroll
-        for (int y = 0; y < WT; ++y) {
-          acc[x][y] = __builtin_amdgcn_mfma_f32_32x32x16_f16(pl[x], qh[y], acc[x][y], 0, 0, 0);
-          acc[x][y] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ph[x], ql[y], acc[x][y], 0, 0, 0);
-          acc[x][y] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ph[x], qh[y], acc[x][y], 0, 0, 0);
-        }
-    }
-  }
+  multiply<BT>(acc, lds, P + (long)ti * BT * pitch + k_lo * 128l, Q + (long)tj * BT * pitch + k_lo * 128l, pitch, nk);
+  const int wi = w >> 1, wj = w & 1, fr = lane & 31, half = lane >> 5;
   // register e of a wave's tile (x, y): row (e & 3) + 8 (e >> 2) + 4 half, column fr
-  if (MODE <= TO_B && nsplit > 1) {
+  if (MODE <= TO_B && BT < 256 && nsplit > 1) {
     float* o = ws_part(q) + ((long)tile * nsplit + part) * (BT * BT) + tid;
 #pragma unroll
-    for (int x = 0; x < WT; ++x)
+    for (int x = 0; x < W; ++x)
 #pragma unroll
-      for (int y = 0; y < WT; ++y)
+      for (int y = 0; y < W; ++y)
 #pragma unroll
-        for (int e = 0; e < 16; ++e) o[((x * WT + y) * 16 + e) * 256] = acc[x][y][e];
+        for (int e = 0; e < 16; ++e) o[((x * W + y) * 16 + e) * 256] = acc[x][y][e];
     return;
   }
   const float mul = result_scale<MODE>(q, step);
-  const int i0 = wi * (BT / 2) + 4 * half, j0 = wj * (BT / 2) + fr;
-  if (MODE >= TO_OUT) {
-    const bool tall = q.rows > q.cols;
-#pragma unroll
-    for (int x = 0; x < WT; ++x)
-#pragma unroll
-      for (int y = 0; y < WT; ++y)
-#pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          const long i = (long)ti * BT + i0 + x * 32 + (e & 3) + 8 * (e >> 2), j = (long)tj * BT + j0 + y * 32;
-          if (i >= q.m || j >= q.n) continue;
-          const float v = acc[x][y][e] * mul;
-          const long at = tall ? j * q.cols + i : i * q.cols + j;
-          if (MODE == TO_OUT) {
-            El<T>::put(q.out, at, v);
-          } else {
-            float* p = static_cast<float*>(q.out);
-            p[at] = fmaf(p[at], decay, -rate * q.adjust * v);
-          }
-        }
-    return;
-  }
-  // the tile and its transpose leave through LDS as rows of pairs
+  const int i0 = wi * W * 32 + 4 * half, j0 = wj * W * 32 + fr;
+  // the tile and its transpose leave through LDS as rows of pairs, 16 bytes a lane
   const bool diag = MODE <= TO_B && ti == tj;
 #pragma unroll
-  for (int x = 0; x < WT; ++x)
+  for (int x = 0; x < W; ++x)
 #pragma unroll
-    for (int y = 0; y < WT; ++y)
+    for (int y = 0; y < W; ++y)
 #pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        float v = acc[x][y][e] * mul;
-        if (diag && i0 + x * 32 + (e & 3) + 8 * (e >> 2) == j0 + y * 32) v += diagonal<MODE>();
-        acc[x][y][e] = v;
+      for (int e = 0; e < 16; ++e) acc[x][y][e] *= mul;
+  constexpr int ROWS = BT / S::PASSES;
+  if (MODE >= TO_OUT) {
+    // results in the orientation of the caller's matrix, as rows of floats through LDS
+    const bool tall = q.rows > q.cols;
+    const long row0 = (long)(tall ? tj : ti) * BT, col0 = (long)(tall ? ti : tj) * BT;
+#pragma unroll
+    for (int p = 0; p < S::PASSES; ++p) {
+      __syncthreads();
+      if (S::PASSES == 1 || (tall ? j0 : i0) / ROWS == p) {
+#pragma unroll
+        for (int x = 0; x < W; ++x)
+#pragma unroll
+          for (int y = 0; y < W; ++y)
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+              const int i = i0 + x * 32 + 8 * g, j = j0 + y * 32;
+              if (tall) {
+                f32x4 v;
+#pragma unroll
+                for (int r = 0; r < 4; ++r) v[r] = acc[x][y][g * 4 + r];
+                *reinterpret_cast<f32x4*>(lds + (j - p * ROWS) * S::OUTROW + i * 4) = v;
+              } else {
+#pragma unroll
+                for (int r = 0; r < 4; ++r)
+                  *reinterpret_cast<float*>(lds + (i + r - p * ROWS) * S::OUTROW + j * 4) = acc[x][y][g * 4 + r];
+              }
+            }
       }
+      __syncthreads();
+      for (int u = tid; u < ROWS * BT / 4; u += 256) {
+        const int r = u / (BT / 4), c = u % (BT / 4) * 4;
+        const long row = row0 + p * ROWS + r, col = col0 + c;
+        if (row >= q.rows || col >= q.cols) continue;
+        const f32x4 v = *reinterpret_cast<const f32x4*>(lds + r * S::OUTROW + c * 4);
+        const long at = row * q.cols + col;
+        const int n = q.cols - col < 4 ? (int)(q.cols - col) : 4;
+        if (MODE == TO_OUT) {
+          if (n == 4)
+            El<T>::put4(q.out, at, v);
+          else
+            for (int k = 0; k < n; ++k) El<T>::put(q.out, at + k, v[k]);
+        } else {
+          float* o = static_cast<float*>(q.out) + at;
+          const float f = -rate * q.adjust;
+          if (n == 4) {
+            f32x4u old = *reinterpret_cast<const f32x4u*>(o);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) old[k] = fmaf(old[k], decay, f * v[k]);
+            *reinterpret_cast<f32x4u*>(o) = old;
+          } else {
+            for (int k = 0; k < n; ++k) o[k] = fmaf(o[k], decay, f * v[k]);
+          }
+        }
+      }
+    }
+    return;
+  }
   char* direct = MODE == TO_T ? ws_t(q) : MODE == TO_B ? ws_b(q) : ws_x(q);
   char* mirror = MODE == TO_X ? ws_xt(q, which ^ 1) : direct;
-  const long dpitch = 4l * (MODE == TO_X ? q.np : q.mp), mpitch = 4l * q.mp;
+  const long dpitch = row_bytes(MODE == TO_X ? q.np : q.mp), mpitch = row_bytes(q.mp);
   auto copy_out = [&](char* dst, long dst_pitch) {
-    for (int u = tid; u < BT * BT / 4; u += 256) {
+    for (int u = tid; u < ROWS * BT / 4; u += 256) {
       const int row = u / (BT / 4), unit = u % (BT / 4);
       *reinterpret_cast<uint4*>(dst + row * dst_pitch + unit * 16) =
-          *reinterpret_cast<const uint4*>(lds + row * OUTROW + unit * 16);
+          *reinterpret_cast<const uint4*>(lds + row * S::OUTROW + unit * 16);
     }
   };
-  __syncthreads();
 #pragma unroll
-  for (int x = 0; x < WT; ++x)
+  for (int p = 0; p < S::PASSES; ++p) {
+    __syncthreads();
+    if (S::PASSES == 1 || i0 / ROWS == p) {
 #pragma unroll
-    for (int y = 0; y < WT; ++y)
+      for (int x = 0; x < W; ++x)
 #pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        const int i = i0 + x * 32 + (e & 3) + 8 * (e >> 2), j = j0 + y * 32;
-        const float v = acc[x][y][e];
+        for (int y = 0; y < W; ++y)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            const int i = i0 - p * ROWS + x * 32 + (e & 3) + 8 * (e >> 2), j = j0 + y * 32;
+            const float v = acc[x][y][e];
+            const _Float16 hi = (_Float16)v;
+            _Float16* o = reinterpret_cast<_Float16*>(lds + i * S::OUTROW + (j >> 4) * 64) + (j & 15);
+            o[0] = hi;
+            o[16] = (_Float16)(v - (float)hi);
+          }
+    }
+    __syncthreads();
+    if (diag) {
+      if (tid < ROWS) {
+        const int j = p * ROWS + tid;
+        _Float16* o = reinterpret_cast<_Float16*>(lds + tid * S::OUTROW + (j >> 4) * 64) + (j & 15);
+        const float v = ((float)o[0] + (float)o[16]) + diagonal<MODE>();
         const _Float16 hi = (_Float16)v;
-        _Float16* o = reinterpret_cast<_Float16*>(lds + i * OUTROW + (j >> 5) * 128) + (j & 31);
         o[0] = hi;
-        o[32] = (_Float16)(v - (float)hi);
+        o[16] = (_Float16)(v - (float)hi);
       }
-  __syncthreads();
-  copy_out(direct + (long)ti * BT * dpitch + tj * (BT * 4l), dpitch);
+      __syncthreads();
+    }
+    copy_out(direct + ((long)ti * BT + p * ROWS) * dpitch + tj * (BT * 4l), dpitch);
+  }
   if (diag) return;
-  __syncthreads();
 #pragma unroll
-  for (int x = 0; x < WT; ++x)
+  for (int p = 0; p < S::PASSES; ++p) {
+    __syncthreads();
+    if (S::PASSES == 1 || j0 / ROWS == p) {
 #pragma unroll
-    for (int y = 0; y < WT; ++y)
+      for (int x = 0; x < W; ++x)
 #pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        const int i = i0 + x * 32 + 8 * g, j = j0 + y * 32;
-        f16x4 hi, lo;
+        for (int y = 0; y < W; ++y)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const float v = acc[x][y][g * 4 + r];
-          hi[r] = (_Float16)v;
-          lo[r] = (_Float16)(v - (float)hi[r]);
-        }
-        char* o = lds + j * OUTROW + (i >> 5) * 128 + (i & 31) * 2;
-        *reinterpret_cast<f16x4*>(o) = hi;
-        *reinterpret_cast<f16x4*>(o + 64) = lo;
-      }
-  __syncthreads();
-  copy_out(mirror + (long)tj * BT * mpitch + ti * (BT * 4l), mpitch);
+          for (int g = 0; g < 4; ++g) {
+            const int i = i0 + x * 32 + 8 * g, j = j0 - p * ROWS + y * 32;
+            f16x4 hi, lo;
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+              const float v = acc[x][y][g * 4 + r];
+              hi[r] = (_Float16)v;
+              lo[r] = (_Float16)(v - (float)hi[r]);
+            }
+            char* o = lds + j * S::OUTROW + (i >> 4) * 64 + (i & 15) * 2;
+            *reinterpret_cast<f16x4*>(o) = hi;
+            *reinterpret_cast<f16x4*>(o + 32) = lo;
+          }
+    }
+    __syncthreads();
+    copy_out(mirror + ((long)tj * BT + p * ROWS) * mpitch + ti * (BT * 4l), mpitch);
+  }
 }
 
 // sums the partial tiles of the matrices whose K was split, one value per thread in the product kernel's register order
 template <int BT, int MODE>
 __global__ __launch_bounds__(256) void join_kernel(const Group* __restrict__ grp, int step) {
-  constexpr int WT = BT / 64, PER = BT * BT / 256;
+  constexpr int W = Tile<BT>::W, PER = BT * BT / 256;
   const Group& gr = *grp;
   const int mi = find_mat(gr.first[PH_JOIN + MODE], gr.count, blockIdx.x);
   const Mat& q = gr.mat[mi];
@@ -425,9 +607,9 @@ __global__ __launch_bounds__(256) void join_kernel(const Group* __restrict__ grp
   float v = 0.f;
   for (int s = 0; s < nsplit; ++s) v += p[(long)s * (BT * BT)];
   v *= result_scale<MODE>(q, step);
-  const int e = r & 15, x = (r >> 4) / WT, y = (r >> 4) % WT, lane = tid & 63, w = tid >> 6;
-  const long i = (long)ti * BT + (w >> 1) * (BT / 2) + x * 32 + (e & 3) + 8 * (e >> 2) + 4 * (lane >> 5);
-  const long j = (long)tj * BT + (w & 1) * (BT / 2) + y * 32 + (lane & 31);
+  const int e = r & 15, x = (r >> 4) / W, y = (r >> 4) % W, lane = tid & 63, w = tid >> 6;
+  const long i = (long)ti * BT + (w >> 1) * W * 32 + x * 32 + (e & 3) + 8 * (e >> 2) + 4 * (lane >> 5);
+  const long j = (long)tj * BT + (w & 1) * W * 32 + y * 32 + (lane & 31);
   if (i == j) v += diagonal<MODE>();
   char* dst = MODE == TO_T ? ws_t(q) : ws_b(q);
   put_pair(dst, i, j, q.mp, v);
@@ -449,59 +631,123 @@ int check_sizes(const int* rows, const int* cols, int count) {
 
 struct Plan {
   int bt[3];       // tile of the T, B and X products
+  int from[GROUP];   // which of the caller's matrices each one is
   int blocks[PH_COUNT];
   long bytes;
 };
 
 long tri(long t) { return t * (t + 1) / 2; }
 
-// Everything that follows from the sizes alone: padding, tiles, splits, the blocks of every launch and the scratch.
-// Tiles are 128 x 128 (a wave's 64 x 64 reads half as much LDS per product as 32 x 32) where a phase then still has
-// ENOUGH tiles to occupy the chip, else 64 x 64; a phase with fewer blocks than that, or with one K much longer than
-// the others', cuts K so that no block has more than its share of TARGET blocks.
-constexpr int ENOUGH = 192, TARGET = 512, MIN_STEPS = 8;
+// What a phase costs in microseconds with BT x BT tiles, from measurements (squares of 256 to 4096 values): a block
+// costs `start` plus `unit` per 32 values of K where it has a compute unit to itself and `full` where the chip is full
+// (64: two blocks share a unit).  Larger tiles read less per product, so they win once they fill the chip.
+struct TileCost {
+  int bt, slots;
+  float start, unit, full;
+};
+constexpr TileCost COST[3] = {{64, 512, 4.0f, 0.27f, 0.54f}, {128, 256, 7.4f, 0.49f, 0.77f}, {256, 256, 9.6f, 2.25f, 2.25f}};
 
+// blocks: how many, their K steps in all, the longest and the shortest of them
+float phase_cost(const TileCost& c, long blocks, long steps, long longest, long shortest) {
+  const float unit = blocks <= 256 ? c.unit + (c.full - c.unit) * (c.bt == 64 ? 0.f : blocks / 256.f) : c.full;
+  float rounds;
+  if (longest == shortest)
+    rounds = (float)((blocks + c.slots - 1) / c.slots);
+  else
+    rounds = (float)steps / c.slots / longest + (blocks <= c.slots ? 0.f : 0.5f);
+  if (rounds < 1.f) rounds = 1.f;
+  return rounds * (c.start + unit * longest);
+}
+
+struct Dims {
+  int m, n;
+};
+
+// Everything that follows from the sizes alone: order (long K first, so that no long block starts last), padding, tiles,
+// splits of K, the blocks of every launch and the scratch.
 void make_plan(const int* rows, const int* cols, Group* gr, Plan* pl) {
   const int n = gr->count;
-  long x128 = 0;
-  for (int i = 0; i < n; ++i)
-    x128 += (long)mmsa_cdiv(rows[i], 128) * mmsa_cdiv(cols[i], 128);
-  const int pad = x128 >= ENOUGH ? 128 : 64;
+  Dims d[GROUP];
+  for (int i = 0; i < n; ++i) {
+    pl->from[i] = i;
+    d[i].m = rows[i] < cols[i] ? rows[i] : cols[i];
+    d[i].n = rows[i] < cols[i] ? cols[i] : rows[i];
+  }
+  for (int i = 1; i < n; ++i)
+    for (int j = i; j > 0 && d[pl->from[j]].n > d[pl->from[j - 1]].n; --j) {
+      const int t = pl->from[j];
+      pl->from[j] = pl->from[j - 1];
+      pl->from[j - 1] = t;
+    }
+  // the general product decides the padding
+  float best = 0.f;
+  int pad = 0;
+  for (const TileCost& c : COST) {
+    long blocks = 0, steps = 0, longest = 0, shortest = 1l << 40;
+    for (int i = 0; i < n; ++i) {
+      const long mt = mmsa_cdiv(d[i].m, c.bt), t = mt * mmsa_cdiv(d[i].n, c.bt), k = mt * c.bt / 32;
+      blocks += t;
+      steps += t * k;
+      if (k > longest) longest = k;
+      if (k < shortest) shortest = k;
+    }
+    const float us = phase_cost(c, blocks, steps, longest, shortest);
+    if (!pad || us < best) best = us, pad = c.bt;
+  }
   int parts = 0;
   for (int i = 0; i < n; ++i) {
     Mat& q = gr->mat[i];
-    q.rows = rows[i];
-    q.cols = cols[i];
-    q.m = rows[i] < cols[i] ? rows[i] : cols[i];
-    q.n = rows[i] < cols[i] ? cols[i] : rows[i];
+    q.rows = rows[pl->from[i]];
+    q.cols = cols[pl->from[i]];
+    q.m = d[pl->from[i]].m;
+    q.n = d[pl->from[i]].n;
     q.mp = (q.m + pad - 1) / pad * pad;
     q.np = (q.n + pad - 1) / pad * pad;
     q.part0 = parts;
-    q.nparts = mmsa_cdiv((long)rows[i] * cols[i], CHUNK);
+    q.nparts = mmsa_cdiv((long)q.rows * q.cols, CHUNK);
     parts += q.nparts;
   }
   pl->bt[TO_X] = pad;
+  // The symmetric products: tile and share of K a block takes.  Partial tiles cost their way through memory and a
+  // second launch.
   for (int ph = TO_T; ph <= TO_B; ++ph) {
-    long t128 = 0, work = 0, longest = 0, tiles = 0;
-    for (int i = 0; i < n; ++i) t128 += tri(gr->mat[i].mp / 128);
-    const int bt = pad == 128 && t128 >= ENOUGH ? 128 : 64;
-    pl->bt[ph] = bt;
-    for (int i = 0; i < n; ++i) {
-      const Mat& q = gr->mat[i];
-      const long t = tri(q.mp / bt), k = (ph == TO_T ? q.np : q.mp) / 32;
-      tiles += t;
-      work += t * k;
-      if (k > longest) longest = k;
+    float least = 0.f;
+    long share = 0;
+    pl->bt[ph] = 0;
+    for (const TileCost& c : COST) {
+      if (c.bt > pad) break;
+      long work = 0, most = 0;
+      for (int i = 0; i < n; ++i) {
+        const long k = (ph == TO_T ? gr->mat[i].np : gr->mat[i].mp) / 32;
+        work += tri(gr->mat[i].mp / c.bt) * k;
+        if (k > most) most = k;
+      }
+      for (int rounds = 0; rounds <= (c.bt == 256 ? 0 : 4); ++rounds) {       // 0: whole
+        long kper = most;
+        if (rounds) {
+          kper = (work / (rounds * c.slots) + 2) & ~1l;
+          if (kper < 4) kper = 4;
+          if (kper >= most) continue;
+        }
+        long blocks = 0, longest = 0, shortest = 1l << 40, parted = 0;
+        for (int i = 0; i < n; ++i) {
+          const long k = (ph == TO_T ? gr->mat[i].np : gr->mat[i].mp) / 32, sp = (k + kper - 1) / kper;
+          const long each = (k + sp - 1) / sp, t = tri(gr->mat[i].mp / c.bt) * sp;
+          blocks += t;
+          if (sp > 1) parted += t;
+          if (each > longest) longest = each;
+          if (each < shortest) shortest = each;
+        }
+        float us = phase_cost(c, blocks, work, longest, shortest);
+        if (parted) us += 5.f + (float)parted * c.bt * c.bt * 8 / 3e6f;
+        if (!pl->bt[ph] || us < least) least = us, pl->bt[ph] = c.bt, share = kper;
+      }
     }
-    long kper = (work + TARGET - 1) / TARGET;
-    if (kper < MIN_STEPS) kper = MIN_STEPS;
-    const bool split = tiles < ENOUGH || longest > 2 * kper;
     for (int i = 0; i < n; ++i) {
       Mat& q = gr->mat[i];
-      const long k = (ph == TO_T ? q.np : q.mp) / 32;
-      int sp = split ? (int)((k + kper - 1) / kper) : 1;
-      const int each = (int)((k + sp - 1) / sp);
-      q.nsplit[ph] = (int)((k + each - 1) / each);       // no block without a step
+      const long k = (ph == TO_T ? q.np : q.mp) / 32, sp = (k + share - 1) / share;
+      const long each = (k / 2 + sp - 1) / sp * 2;            // an even number of steps
+      q.nsplit[ph] = (int)((k + each - 1) / each);            // no block without a step
     }
   }
   int total[PH_COUNT] = {0};
@@ -524,7 +770,7 @@ void make_plan(const int* rows, const int* cols, Group* gr, Plan* pl) {
       }
     }
     total[PH_PRODUCT + TO_X] += (q.mp / pad) * (q.np / pad);
-    bytes += 3 * xbytes(q) + 2 * sbytes(q) + 128 + 4 * part_floats;
+    bytes += mat_bytes(q) + 4 * part_floats;
   }
   for (int p = 0; p < PH_COUNT; ++p) pl->blocks[p] = total[p];
   pl->bytes = bytes;
@@ -540,11 +786,13 @@ struct Step {
 template <typename T, int MODE>
 void launch_product(const Plan& pl, const Group* dev, int step, const Step& st, hipStream_t s) {
   constexpr int PHASE = MODE < TO_X ? MODE : TO_X;
-  const dim3 grid(pl.blocks[PH_PRODUCT + PHASE]), block(256);
-  if (pl.bt[PHASE] == 128)
-    hipLaunchKernelGGL((product_kernel<T, 128, MODE>), grid, block, 0, s, dev, step, step & 1, st.decay, st.rate);
+  const dim3 grid(pl.blocks[PH_PRODUCT + PHASE]);
+  if (pl.bt[PHASE] == 256)
+    hipLaunchKernelGGL((product_kernel<T, 256, MODE>), grid, dim3(256), 0, s, dev, step, step & 1, st.decay, st.rate);
+  else if (pl.bt[PHASE] == 128)
+    hipLaunchKernelGGL((product_kernel<T, 128, MODE>), grid, dim3(256), 0, s, dev, step, step & 1, st.decay, st.rate);
   else
-    hipLaunchKernelGGL((product_kernel<T, 64, MODE>), grid, block, 0, s, dev, step, step & 1, st.decay, st.rate);
+    hipLaunchKernelGGL((product_kernel<T, 64, MODE>), grid, dim3(256), 0, s, dev, step, step & 1, st.decay, st.rate);
 }
 template <int MODE>
 void launch_join(const Plan& pl, const Group* dev, int step, hipStream_t s) {
@@ -567,9 +815,10 @@ int run_all(const void* const* src, void* const* dst, void* const* mom, const in
     make_plan(rows + i0, cols + i0, &gr, &pl);
     for (int i = 0; i < gr.count; ++i) {
       Mat& q = gr.mat[i];
-      q.g = src[i0 + i];
-      q.out = dst[i0 + i];
-      q.mom = mom ? static_cast<float*>(mom[i0 + i]) : nullptr;
+      const int at = i0 + pl.from[i];
+      q.g = src[at];
+      q.out = dst[at];
+      q.mom = mom ? static_cast<float*>(mom[at]) : nullptr;
       q.ws = static_cast<char*>(scratch) + q.ws_off;
       q.adjust = q.rows > q.cols ? sqrtf((float)q.rows / (float)q.cols) : 1.f;
     }
