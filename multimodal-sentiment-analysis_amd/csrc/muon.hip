@@ -36,7 +36,6 @@ constexpr float NS_SHIFT = (float)(-4.775 / (2.0 * 2.0315)), NS_REST = (float)(3
 constexpr int NS_SCALE = 14;           // log2 of the fixed-point scale
 constexpr int MAX_STEPS = 16;
 constexpr int GROUP = 24;              // matrices of one launch (their descriptors travel as kernel arguments)
-constexpr int CHUNK = 16384;           // values of one partial sum of squares
 
 enum { PH_SUMSQ = 0, PH_SPLIT = 1, PH_PRODUCT = 2 /* T, B, X */, PH_JOIN = 5 /* T, B */, PH_COUNT = 7 };
 
@@ -49,10 +48,10 @@ struct Mat {
   int rows, cols;
   int m, n;             // the smaller and the larger of the two
   int mp, np;           // padded to the tile
-  int part0, nparts;    // its partial sums of squares
+  int part0, nparts;    // its partial sums of squares, `chunk` values each
+  int chunk;
   int nsplit[2];        // blocks that share the K range of a tile of T / B
   float adjust;         // max(1, rows / cols)^1/2
-  int pad_;
 };
 // The descriptors of one set of launches: an argument of the first kernel, which leaves them at the start of the
 // scratch for the others (an argument of this size costs the host a few microseconds per launch).
@@ -92,6 +91,10 @@ typedef unsigned u32x2u __attribute__((ext_vector_type(2), aligned(2)));
 template <typename T> struct El;
 template <> struct El<float> {
   static __device__ __forceinline__ float get(const void* p, long i) { return static_cast<const float*>(p)[i]; }
+  static __device__ __forceinline__ f32x4 get4(const void* p, long i) {
+    const f32x4u u = *reinterpret_cast<const f32x4u*>(static_cast<const float*>(p) + i);
+    return f32x4{u[0], u[1], u[2], u[3]};
+  }
   static __device__ __forceinline__ void put(void* p, long i, float v) { static_cast<float*>(p)[i] = v; }
   static __device__ __forceinline__ void put4(void* p, long i, f32x4 v) {
     f32x4u u = {v[0], v[1], v[2], v[3]};
@@ -101,6 +104,11 @@ template <> struct El<float> {
 template <> struct El<__hip_bfloat16> {
   static __device__ __forceinline__ float get(const void* p, long i) {
     return __uint_as_float((unsigned)static_cast<const unsigned short*>(p)[i] << 16);
+  }
+  static __device__ __forceinline__ f32x4 get4(const void* p, long i) {
+    const u32x2u u = *reinterpret_cast<const u32x2u*>(static_cast<const unsigned short*>(p) + i);
+    return f32x4{__uint_as_float(u[0] << 16), __uint_as_float(u[0] & 0xffff0000u), __uint_as_float(u[1] << 16),
+                 __uint_as_float(u[1] & 0xffff0000u)};
   }
   static __device__ __forceinline__ void put(void* p, long i, float v) {
     static_cast<__hip_bfloat16*>(p)[i] = __float2bfloat16(v);
@@ -116,6 +124,12 @@ template <> struct El<_Float16> {
   static __device__ __forceinline__ float get(const void* p, long i) {
     return (float)static_cast<const _Float16*>(p)[i];
   }
+  static __device__ __forceinline__ f32x4 get4(const void* p, long i) {
+    const u32x2u u = *reinterpret_cast<const u32x2u*>(static_cast<const _Float16*>(p) + i);
+    _Float16 h[4];
+    __builtin_memcpy(h, &u, 8);
+    return f32x4{(float)h[0], (float)h[1], (float)h[2], (float)h[3]};
+  }
   static __device__ __forceinline__ void put(void* p, long i, float v) { static_cast<_Float16*>(p)[i] = (_Float16)v; }
   static __device__ __forceinline__ void put4(void* p, long i, f32x4 v) {
     _Float16 h[4] = {(_Float16)v[0], (_Float16)v[1], (_Float16)v[2], (_Float16)v[3]};
@@ -129,7 +143,7 @@ __device__ __forceinline__ float direction(float g, float mom, float mu, int nes
   return nesterov ? fmaf(mu, mom - g, g) : mom;
 }
 
-// momentum update (MOM) and the sum of squares of u, one block per CHUNK values
+// momentum update (MOM) and the sum of squares of u, one block per chunk
 template <typename T, bool MOM>
 __global__ __launch_bounds__(256) void momentum_sumsq_kernel(const Group gr, float mu, float one_minus_mu, int nesterov,
                                                              double* __restrict__ parts, Group* __restrict__ dev) {
@@ -141,16 +155,33 @@ __global__ __launch_bounds__(256) void momentum_sumsq_kernel(const Group gr, flo
   const int i = find_mat(gr.first[PH_SUMSQ], gr.count, blockIdx.x);
   const Mat& q = gr.mat[i];
   const int c = blockIdx.x - gr.first[PH_SUMSQ][i];
-  const long lo = (long)c * CHUNK, total = (long)q.rows * q.cols;
-  const long hi = lo + CHUNK < total ? lo + CHUNK : total;
+  const long lo = (long)c * q.chunk, total = (long)q.rows * q.cols;
+  const int n = (int)(total - lo < q.chunk ? total - lo : q.chunk), n4 = n & ~3;
+  const T* g = static_cast<const T*>(q.g) + lo;
+  float* mom = MOM ? q.mom + lo : nullptr;
   double ss = 0.0;
-  for (long j = lo + threadIdx.x; j < hi; j += 256) {
-    float u = El<T>::get(q.g, j);
+#pragma unroll 4
+  for (int j = 4 * threadIdx.x; j < n4; j += 1024) {
+    f32x4 u = El<T>::get4(g, j);
     if (MOM) {
-      const float g = u;
-      const float m = fmaf(one_minus_mu, g - q.mom[j], q.mom[j]);
-      q.mom[j] = m;
-      u = direction(g, m, mu, nesterov);
+      f32x4u m = *reinterpret_cast<const f32x4u*>(mom + j);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        m[k] = fmaf(one_minus_mu, u[k] - m[k], m[k]);
+        u[k] = direction(u[k], m[k], mu, nesterov);
+      }
+      *reinterpret_cast<f32x4u*>(mom + j) = m;
+    }
+#pragma unroll
+    for (int k = 0; k < 4; ++k) ss += (double)u[k] * (double)u[k];
+  }
+  if ((int)threadIdx.x < n - n4) {
+    const int j = n4 + threadIdx.x;
+    float u = El<T>::get(g, j);
+    if (MOM) {
+      const float m = fmaf(one_minus_mu, u - mom[j], mom[j]);
+      mom[j] = m;
+      u = direction(u, m, mu, nesterov);
     }
     ss += (double)u * (double)u;
   }
@@ -171,7 +202,8 @@ __device__ __forceinline__ int extra_scale(double r) {
   return min(400, max(0, (int)floor(-log2(r))));
 }
 
-// normalises u and writes X and X^T as pairs, 64 x 64 values of u's padded extent per block
+// normalises u and writes X and X^T as pairs, 64 x 64 values of u's padded extent per block, 16 bytes a lane: sixteen
+// lanes write 256 consecutive bytes of a row
 template <typename T, bool MOM>
 __global__ __launch_bounds__(256) void split_kernel(const Group* __restrict__ grp, float mu, int nesterov, float eps,
                                                     int steps, const double* __restrict__ parts) {
@@ -181,6 +213,34 @@ __global__ __launch_bounds__(256) void split_kernel(const Group* __restrict__ gr
   const int i = find_mat(gr.first[PH_SPLIT], gr.count, blockIdx.x);
   const Mat& q = gr.mat[i];
   const int b = blockIdx.x - gr.first[PH_SPLIT][i];
+  const bool tall = q.rows > q.cols;
+  const int pr = tall ? q.np : q.mp, pc = tall ? q.mp : q.np;      // padded extent in u's own orientation
+  const int nct = pc / 64;
+  const long r0 = (long)(b / nct) * 64, c0 = (long)(b % nct) * 64;
+  // the values first, so that they arrive while the norm is added up
+  float u[4][4];
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const long row = r0 + (threadIdx.x >> 4) + 16 * k, col = c0 + (threadIdx.x & 15) * 4;
+    const long at = row * q.cols + col;
+    const int n = row >= q.rows || col >= q.cols ? 0 : q.cols - col < 4 ? (int)(q.cols - col) : 4;
+    if (n == 4) {
+      const f32x4 v = El<T>::get4(q.g, at);
+      f32x4u m{};
+      if (MOM) m = *reinterpret_cast<const f32x4u*>(q.mom + at);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) u[k][e] = MOM ? direction(v[e], m[e], mu, nesterov) : v[e];
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        u[k][e] = 0.f;
+        if (e < n) {
+          u[k][e] = El<T>::get(q.g, at + e);
+          if (MOM) u[k][e] = direction(u[k][e], q.mom[at + e], mu, nesterov);
+        }
+      }
+    }
+  }
   double ss = 0.0;
   for (int j = threadIdx.x; j < q.nparts; j += 256) ss += parts[q.part0 + j];
   ss = block_sum_d(ss, red);
@@ -196,27 +256,29 @@ __global__ __launch_bounds__(256) void split_kernel(const Group* __restrict__ gr
     }
   }
   const double mul = ldexp(1.0 / size, NS_SCALE + k0);
-  const bool tall = q.rows > q.cols;
-  const int pr = tall ? q.np : q.mp, pc = tall ? q.mp : q.np;      // padded extent in u's own orientation
-  const int nct = pc / 64;
-  const long r0 = (long)(b / nct) * 64, c0 = (long)(b % nct) * 64;
+#pragma unroll
+  for (int k = 0; k < 4; ++k)
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      tile[(threadIdx.x >> 4) + 16 * k][(threadIdx.x & 15) * 4 + e] = (float)((double)u[k][e] * mul);
+  __syncthreads();
   char* rowm = tall ? ws_xt(q, 0) : ws_x(q);                       // [pr][pc]
   char* colm = tall ? ws_x(q) : ws_xt(q, 0);                       // [pc][pr]
-  const int tx = threadIdx.x & 63, ty = threadIdx.x >> 6;
-  for (int rr = ty; rr < 64; rr += 4) {
-    const long row = r0 + rr, col = c0 + tx;
-    float v = 0.f;
-    if (row < q.rows && col < q.cols) {
-      const long at = row * q.cols + col;
-      float u = El<T>::get(q.g, at);
-      if (MOM) u = direction(u, q.mom[at], mu, nesterov);
-      v = (float)((double)u * mul);
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const int line = (threadIdx.x >> 4) + 16 * k, unit = threadIdx.x & 15;
+    const int at = (unit >> 2) * 16 + (unit & 1) * 8;              // units of a run: hi, hi, lo, lo
+    f16x8 o, t;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const float v = tile[line][at + e], c = tile[at + e][line];
+      const _Float16 hv = (_Float16)v, hc = (_Float16)c;
+      o[e] = unit & 2 ? (_Float16)(v - (float)hv) : hv;
+      t[e] = unit & 2 ? (_Float16)(c - (float)hc) : hc;
     }
-    tile[rr][tx] = v;
-    put_pair(rowm, row, col, pc, v);
+    *reinterpret_cast<f16x8*>(rowm + (r0 + line) * row_bytes(pc) + c0 * 4 + unit * 16) = o;
+    *reinterpret_cast<f16x8*>(colm + (c0 + line) * row_bytes(pr) + r0 * 4 + unit * 16) = t;
   }
-  __syncthreads();
-  for (int cc = ty; cc < 64; cc += 4) put_pair(colm, c0 + cc, r0 + tx, pr, tile[tx][cc]);
 }
 
 // ---- products
@@ -591,29 +653,53 @@ __global__ __launch_bounds__(256, BT == 256 || Tile<BT>::LDS > 81920 ? 1 : 2) vo
   }
 }
 
-// sums the partial tiles of the matrices whose K was split, one value per thread in the product kernel's register order
+// Sums the partial tiles of the matrices whose K was split, four values (of one column) per lane.  Many parts are shared
+// out among a block's four waves; of few parts every wave adds up its own values.
+__host__ __device__ inline bool many_parts(int nsplit) { return nsplit >= 8; }
+
 template <int BT, int MODE>
 __global__ __launch_bounds__(256) void join_kernel(const Group* __restrict__ grp, int step) {
-  constexpr int W = Tile<BT>::W, PER = BT * BT / 256;
+  constexpr int W = Tile<BT>::W, PER = BT * BT / 256;          // groups of 64 x 4 values in a tile
+  __shared__ f32x4 sums[4][64];
   const Group& gr = *grp;
   const int mi = find_mat(gr.first[PH_JOIN + MODE], gr.count, blockIdx.x);
   const Mat& q = gr.mat[mi];
-  const int b = blockIdx.x - gr.first[PH_JOIN + MODE][mi];
-  const int tile = b / PER, r = b % PER, tid = threadIdx.x;
+  const int b = blockIdx.x - gr.first[PH_JOIN + MODE][mi], lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int nsplit = q.nsplit[MODE];
+  const bool many = many_parts(nsplit);
+  const int unit = many ? b : b * 4 + wave, tile = unit / PER, r = unit % PER;
+  const int w = r & 3, g = (r >> 2) & 3, x = (r >> 4) / W, y = (r >> 4) % W;
+  const float* p = ws_part(q) + (long)tile * nsplit * (BT * BT) + ((x * W + y) * 16 + 4 * g) * 256 + w * 64 + lane;
+  f32x4 v = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+  for (int s = many ? wave : 0; s < nsplit; s += many ? 4 : 1)
+#pragma unroll
+    for (int k = 0; k < 4; ++k) v[k] += p[(long)s * (BT * BT) + k * 256];
+  if (many) {
+    sums[wave][lane] = v;
+    __syncthreads();
+    if (wave) return;
+    v = (sums[0][lane] + sums[1][lane]) + (sums[2][lane] + sums[3][lane]);
+  }
   int ti, tj;
   lower_tile(tile, ti, tj);
-  const float* p = ws_part(q) + (long)tile * nsplit * (BT * BT) + r * 256 + tid;
-  float v = 0.f;
-  for (int s = 0; s < nsplit; ++s) v += p[(long)s * (BT * BT)];
-  v *= result_scale<MODE>(q, step);
-  const int e = r & 15, x = (r >> 4) / W, y = (r >> 4) % W, lane = tid & 63, w = tid >> 6;
-  const long i = (long)ti * BT + (w >> 1) * W * 32 + x * 32 + (e & 3) + 8 * (e >> 2) + 4 * (lane >> 5);
+  const float mul = result_scale<MODE>(q, step);
+  const long i = (long)ti * BT + (w >> 1) * W * 32 + x * 32 + 8 * g + 4 * (lane >> 5);
   const long j = (long)tj * BT + (w & 1) * W * 32 + y * 32 + (lane & 31);
-  if (i == j) v += diagonal<MODE>();
   char* dst = MODE == TO_T ? ws_t(q) : ws_b(q);
-  put_pair(dst, i, j, q.mp, v);
-  if (ti != tj) put_pair(dst, j, i, q.mp, v);
+  f16x4 hi, lo;
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    float o = v[k] * mul;
+    if (i + k == j) o += diagonal<MODE>();
+    hi[k] = (_Float16)o;
+    lo[k] = (_Float16)(o - (float)hi[k]);
+    put_pair(dst, i + k, j, q.mp, o);
+  }
+  if (ti == tj) return;
+  char* o = dst + j * row_bytes(q.mp) + (i >> 4) * 64 + (i & 15) * 2;
+  *reinterpret_cast<f16x4*>(o) = hi;
+  *reinterpret_cast<f16x4*>(o + 32) = lo;
 }
 
 // ---- host side
@@ -704,7 +790,11 @@ void make_plan(const int* rows, const int* cols, Group* gr, Plan* pl) {
     q.mp = (q.m + pad - 1) / pad * pad;
     q.np = (q.n + pad - 1) / pad * pad;
     q.part0 = parts;
-    q.nparts = mmsa_cdiv((long)q.rows * q.cols, CHUNK);
+    // at most 512 partial sums: every block of the next kernel adds all of them up
+    const long values = (long)q.rows * q.cols;
+    q.chunk = (int)((values + 511) / 512 + 3) & ~3;
+    if (q.chunk < 4096) q.chunk = 4096;
+    q.nparts = mmsa_cdiv(values, q.chunk);
     parts += q.nparts;
   }
   pl->bt[TO_X] = pad;
@@ -729,17 +819,18 @@ void make_plan(const int* rows, const int* cols, Group* gr, Plan* pl) {
           if (kper < 4) kper = 4;
           if (kper >= most) continue;
         }
-        long blocks = 0, longest = 0, shortest = 1l << 40, parted = 0;
+        long blocks = 0, longest = 0, shortest = 1l << 40, parted = 0, parts = 0;
         for (int i = 0; i < n; ++i) {
           const long k = (ph == TO_T ? gr->mat[i].np : gr->mat[i].mp) / 32, sp = (k + kper - 1) / kper;
           const long each = (k + sp - 1) / sp, t = tri(gr->mat[i].mp / c.bt) * sp;
           blocks += t;
           if (sp > 1) parted += t;
+          if (sp > parts) parts = sp;
           if (each > longest) longest = each;
           if (each < shortest) shortest = each;
         }
         float us = phase_cost(c, blocks, work, longest, shortest);
-        if (parted) us += 5.f + (float)parted * c.bt * c.bt * 8 / 3e6f;
+        if (parted) us += 5.f + 0.04f * parts + (float)parted * c.bt * c.bt * 8 / 3e6f;
         if (!pl->bt[ph] || us < least) least = us, pl->bt[ph] = c.bt, share = kper;
       }
     }
@@ -764,7 +855,7 @@ void make_plan(const int* rows, const int* cols, Group* gr, Plan* pl) {
       const long t = tri(q.mp / bt);
       total[PH_PRODUCT + ph] += (int)(t * q.nsplit[ph]);
       if (q.nsplit[ph] > 1) {
-        total[PH_JOIN + ph] += (int)(t * (bt * bt / 256));
+        total[PH_JOIN + ph] += (int)(t * (bt * bt / (many_parts(q.nsplit[ph]) ? 256 : 1024)));
         const long f = t * q.nsplit[ph] * bt * bt;
         if (f > part_floats) part_floats = f;
       }
