@@ -11,99 +11,103 @@
 // That holds for any C, odd ones too, so there is one code path with 16-byte accesses (a sample may start at any value:
 // the vectors are declared with the alignment of one value, which this target's global accesses allow).
 #include "mmsa_common.h"
-#include <hip/hip_bf16.h>
-#include <hip/hip_fp16.h>
 
 namespace {
 
 enum { ACT_NONE = 0, ACT_RELU = 1, ACT_SILU = 2, ACT_GELU = 3 };
 
 typedef unsigned u32x4a __attribute__((ext_vector_type(4), aligned(2)));
-typedef float f32x4a __attribute__((ext_vector_type(4), aligned(4)));
+typedef unsigned u32x2a __attribute__((ext_vector_type(2), aligned(2)));
+typedef unsigned u32a __attribute__((aligned(2)));
 
+// 16-bit values travel as raw bits
+struct bf16_t { unsigned short b; };
+struct fp16_t { _Float16 h; };
+__device__ __forceinline__ unsigned short f32_to_bf16(float f) {
+  const __bf16 h = (__bf16)f;               // round to nearest even, one conversion instruction for two values
+  unsigned short u;
+  __builtin_memcpy(&u, &h, 2);
+  return u;
+}
 template <typename T> struct Io;
 template <> struct Io<float> {
   static constexpr int V = 4;
   static __device__ __forceinline__ float to(float v) { return v; }
   static __device__ __forceinline__ float from(float v) { return v; }
-  static __device__ __forceinline__ void load(const float* p, float (&o)[4]) {
-    const f32x4a r = *reinterpret_cast<const f32x4a*>(p);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) o[i] = r[i];
-  }
-  static __device__ __forceinline__ void store(float* p, const float (&o)[4]) {
-    f32x4a r;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) r[i] = o[i];
-    *reinterpret_cast<f32x4a*>(p) = r;
-  }
 };
-// 16-bit values travel as raw bits
-__device__ __forceinline__ float bf16_to_f32(unsigned short b) { return __uint_as_float((unsigned)b << 16); }
-__device__ __forceinline__ unsigned short f32_to_bf16(float f) {
-  __hip_bfloat16 h = __float2bfloat16(f);   // round to nearest even
-  unsigned short u;
-  __builtin_memcpy(&u, &h, 2);
-  return u;
-}
-struct bf16_t { unsigned short b; };
-struct fp16_t { _Float16 h; };
 template <> struct Io<bf16_t> {
   static constexpr int V = 8;
-  static __device__ __forceinline__ float to(bf16_t v) { return bf16_to_f32(v.b); }
+  static __device__ __forceinline__ float to(bf16_t v) { return __uint_as_float((unsigned)v.b << 16); }
   static __device__ __forceinline__ bf16_t from(float v) { return bf16_t{f32_to_bf16(v)}; }
-  static __device__ __forceinline__ void load(const bf16_t* p, float (&o)[8]) {
-    const u32x4a r = *reinterpret_cast<const u32x4a*>(p);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      o[2 * i] = __uint_as_float(r[i] << 16);
-      o[2 * i + 1] = __uint_as_float(r[i] & 0xffff0000u);
-    }
-  }
-  static __device__ __forceinline__ void store(bf16_t* p, const float (&o)[8]) {
-    u32x4a r;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) r[i] = (unsigned)f32_to_bf16(o[2 * i]) | ((unsigned)f32_to_bf16(o[2 * i + 1]) << 16);
-    *reinterpret_cast<u32x4a*>(p) = r;
-  }
 };
 template <> struct Io<fp16_t> {
   static constexpr int V = 8;
   static __device__ __forceinline__ float to(fp16_t v) { return (float)v.h; }
   static __device__ __forceinline__ fp16_t from(float v) { return fp16_t{(_Float16)v}; }
-  static __device__ __forceinline__ void load(const fp16_t* p, float (&o)[8]) {
-    const u32x4a r = *reinterpret_cast<const u32x4a*>(p);
-    _Float16 h[8];
-    __builtin_memcpy(h, &r, 16);
+};
+
+// W values as they lie in memory (2 to 16 bytes), and their 32-bit values
+template <int BYTES> struct Bits;
+template <> struct Bits<16> { typedef u32x4a type; };
+template <> struct Bits<8> { typedef u32x2a type; };
+template <> struct Bits<4> { typedef u32a type; };
+template <> struct Bits<2> { typedef unsigned short type; };
+template <typename T, int W> struct Pack {
+  typename Bits<W * (int)sizeof(T)>::type raw;
+  __device__ __forceinline__ void load(const T* p) { raw = *reinterpret_cast<const decltype(raw)*>(p); }
+  __device__ __forceinline__ void store(T* p) const { *reinterpret_cast<decltype(raw)*>(p) = raw; }
+  __device__ __forceinline__ void get(float (&o)[W]) const {
+    T v[W];
+    __builtin_memcpy(v, &raw, W * sizeof(T));
 #pragma unroll
-    for (int i = 0; i < 8; ++i) o[i] = (float)h[i];
+    for (int i = 0; i < W; ++i) o[i] = Io<T>::to(v[i]);
   }
-  static __device__ __forceinline__ void store(fp16_t* p, const float (&o)[8]) {
-    _Float16 h[8];
+  __device__ __forceinline__ void set(const float (&o)[W]) {
+    T v[W];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) h[i] = (_Float16)o[i];
-    u32x4a r;
-    __builtin_memcpy(&r, h, 16);
-    *reinterpret_cast<u32x4a*>(p) = r;
+    for (int i = 0; i < W; ++i) v[i] = Io<T>::from(o[i]);
+    __builtin_memcpy(&raw, v, W * sizeof(T));
   }
 };
 
+// The kernels on 16-bit maps are bound by the vector unit as much as by memory, so the activations are written for few
+// instructions: the hardware's exponential and reciprocal (each good to about 1 unit of float32), and for GELU
+//   Phi(z) = 1 - e P(t) for z >= 0, e P(t) for z < 0,  e = exp(-z^2 / 2),  t = 1 / (1 + p |z| / sqrt 2)
+// (Abramowitz and Stegun 7.1.26, 0.75e-7 off at most), which shares its exponential with the density in the slope.
+__device__ __forceinline__ float fast_exp(float x) { return __builtin_amdgcn_exp2f(x * 1.44269504088896341f); }
+__device__ __forceinline__ float sigmoid(float z) { return __builtin_amdgcn_rcpf(1.f + fast_exp(-z)); }
+__device__ __forceinline__ float normal_cdf(float z, float& e) {
+  e = fast_exp(-0.5f * z * z);
+  const float t = __builtin_amdgcn_rcpf(fmaf(0.3275911f * 0.70710678118654752f, fabsf(z), 1.f));
+  float p = fmaf(t, 0.5f * 1.061405429f, 0.5f * -1.453152027f);
+  p = fmaf(t, p, 0.5f * 1.421413741f);
+  p = fmaf(t, p, 0.5f * -0.284496736f);
+  p = fmaf(t, p, 0.5f * 0.254829592f);
+  p *= t * e;
+  return z < 0.f ? p : 1.f - p;
+}
 template <int ACT>
 __device__ __forceinline__ float act_fwd(float z) {
   if (ACT == ACT_RELU) return z < 0.f ? 0.f : z;      // NaN stays NaN
-  if (ACT == ACT_SILU) return z / (1.f + __expf(-z));
-  if (ACT == ACT_GELU) return 0.5f * z * (1.f + erff(z * 0.70710678118654752f));
+  if (ACT == ACT_SILU) return z * sigmoid(z);
+  if (ACT == ACT_GELU) {
+    float e;
+    return z * normal_cdf(z, e);
+  }
   return z;
 }
 template <int ACT>
 __device__ __forceinline__ float act_slope(float z) {
   if (ACT == ACT_RELU) return z > 0.f ? 1.f : 0.f;
   if (ACT == ACT_SILU) {
-    const float s = 1.f / (1.f + __expf(-z));
+    const float s = sigmoid(z);
     return s * fmaf(z, 1.f - s, 1.f);
   }
-  if (ACT == ACT_GELU)
-    return fmaf(z * 0.39894228040143268f, __expf(-0.5f * z * z), 0.5f * (1.f + erff(z * 0.70710678118654752f)));
+  if (ACT == ACT_GELU) {
+    float e;
+    const float c = normal_cdf(z, e);
+    return fmaf(z * 0.39894228040143268f, e, c);
+  }
   return 1.f;
 }
 
@@ -117,7 +121,33 @@ struct Cut {
   int row;         // vectors from one row of threads to the next (active where columns == 1, else period)
   int iters;
   long nchunk;     // chunks per sample
+  int team;        // lanes that join the statistics of a group, a power of two up to a wave
 };
+
+// sum over aligned teams of `team` lanes, the same in every lane of a team
+__device__ __forceinline__ double team_sum(double v, int team) {
+  for (int s = 1; s < team; s <<= 1) v += __shfl_xor(v, s);
+  return v;
+}
+
+// a thread's share of a chunk: `full` whole vectors, `row` apart, from the first on; then possibly the sample's last,
+// shorter one
+struct Share {
+  long at;      // first value
+  int full;
+  int rest;     // values of the short vector behind them, 0: none
+};
+template <int V>
+__device__ __forceinline__ Share share_of(const Cut& cut, long ch, int t) {
+  const long v0 = ch * cut.iters * (long)cut.row + t, whole = cut.S / V;
+  Share s;
+  s.at = v0 * V;
+  long n = v0 < whole ? (whole - v0 + cut.row - 1) / cut.row : 0;
+  if (n > cut.iters) n = cut.iters;
+  s.full = (int)n;
+  s.rest = n < cut.iters && v0 + n * cut.row == whole ? (int)(cut.S - whole * V) : 0;
+  return s;
+}
 
 // ---------------------------------------------------------------------------------------------------- statistics
 // Every thread sums d = x - k and d^2 per channel, k being its own first value: as k is one of the values summed, the
@@ -127,7 +157,7 @@ struct Cut {
 template <typename T>
 __global__ __launch_bounds__(1024) void gn_stats_kernel(const T* __restrict__ x, const Cut cut,
                                                         double* __restrict__ part) {
-  constexpr int V = Io<T>::V;
+  constexpr int V = Io<T>::V, U = 4;            // U loads in flight per thread
   extern __shared__ float sh[];                 // [3][slots]: mean, M2, count of every (thread, element)
   const int tid = threadIdx.x;
   const long b = blockIdx.x / cut.nchunk, ch = blockIdx.x % cut.nchunk;
@@ -139,72 +169,87 @@ __global__ __launch_bounds__(1024) void gn_stats_kernel(const T* __restrict__ x,
   for (int col = 0; col < cut.columns; ++col) {
     const int t = col * cut.active + tid;
     if (tid >= cut.active || t >= cut.row) continue;
+    const Share me = share_of<V>(cut, ch, t);
+    const T* p = xs + me.at;
+    const long hop = (long)cut.row * V;
     float k[V], s[V], q[V];
-    int cnt[V];
 #pragma unroll
-    for (int e = 0; e < V; ++e) k[e] = s[e] = q[e] = 0.f, cnt[e] = 0;
-    const long v0 = ch * cut.iters * (long)cut.row + t;
-    for (int it = 0; it < cut.iters; ++it) {
-      const long v = v0 + it * (long)cut.row;
-      if (v >= cut.nvec) break;
-      const long at = v * V;
-      float f[V];
-      if (at + V <= cut.S) {
-        Io<T>::load(xs + at, f);
-        if (it == 0) {
+    for (int e = 0; e < V; ++e) k[e] = s[e] = q[e] = 0.f;
+    if (me.full) {
+      Pack<T, V> f;
+      f.load(p);
+      f.get(k);
+    }
+    int it = 0;
+    for (; it + U <= me.full; it += U, p += U * hop) {
+      Pack<T, V> f[U];
 #pragma unroll
-          for (int e = 0; e < V; ++e) k[e] = f[e];
-        }
+      for (int u = 0; u < U; ++u) f[u].load(p + u * hop);
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        float v[V];
+        f[u].get(v);
 #pragma unroll
         for (int e = 0; e < V; ++e) {
-          const float d = f[e] - k[e];
+          const float d = v[e] - k[e];
           s[e] += d;
           q[e] = fmaf(d, d, q[e]);
-          ++cnt[e];
         }
-      } else {
-        for (int e = 0; e < (int)(cut.S - at); ++e) {
-          const float fe = Io<T>::to(xs[at + e]);
-          if (it == 0) k[e] = fe;
-          const float d = fe - k[e];
-          s[e] += d;
-          q[e] = fmaf(d, d, q[e]);
-          ++cnt[e];
-        }
+      }
+    }
+    for (; it < me.full; ++it, p += hop) {
+      Pack<T, V> f;
+      f.load(p);
+      float v[V];
+      f.get(v);
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        const float d = v[e] - k[e];
+        s[e] += d;
+        q[e] = fmaf(d, d, q[e]);
       }
     }
 #pragma unroll
     for (int e = 0; e < V; ++e) {
-      const float n = (float)cnt[e];
-      const float m = cnt[e] ? s[e] / n : 0.f;
+      if (e < me.rest) {
+        const float v = Io<T>::to(p[e]);
+        if (!me.full) k[e] = v;
+        const float d = v - k[e];
+        s[e] += d;
+        q[e] = fmaf(d, d, q[e]);
+      }
+      const float n = (float)(me.full + (e < me.rest ? 1 : 0));
+      const float m = n > 0.f ? s[e] / n : 0.f;
       smean[t * V + e] = k[e] + m;
       sm2[t * V + e] = fmaxf(fmaf(-s[e], m, q[e]), 0.f);
       scnt[t * V + e] = n;
     }
   }
   __syncthreads();
-  // one wave per group, round robin; slot q belongs to channel q % C (slots is a multiple of C)
-  const int lane = tid & 63, w = tid >> 6, nw = blockDim.x >> 6;
-  const int reps = slots / cut.C;
-  const int per = reps * cut.Cg;
-  for (int g = w; g < cut.G; g += nw) {
+  // a team of lanes per group, all groups at once where there are enough threads; slot q belongs to channel q % C
+  // (slots is a multiple of C)
+  const int per = slots / cut.C * cut.Cg;
+  const int lane = tid & (cut.team - 1), teams = blockDim.x / cut.team;
+  for (int g0 = 0; g0 < cut.G; g0 += teams) {          // uniform: all lanes take part in the sums
+    const int g = g0 + tid / cut.team;
+    const bool mine = g < cut.G;
     double n = 0.0, sum = 0.0;
-    for (int i = lane; i < per; i += 64) {
+    for (int i = lane; mine && i < per; i += cut.team) {
       const int q = (i / cut.Cg) * cut.C + g * cut.Cg + i % cut.Cg;
       n += (double)scnt[q];
       sum += (double)scnt[q] * (double)smean[q];
     }
-    n = wave_sum_d(n);
-    sum = wave_sum_d(sum);
+    n = team_sum(n, cut.team);
+    sum = team_sum(sum, cut.team);
     const double mean = n > 0.0 ? sum / n : 0.0;
     double m2 = 0.0;
-    for (int i = lane; i < per; i += 64) {
+    for (int i = lane; mine && i < per; i += cut.team) {
       const int q = (i / cut.Cg) * cut.C + g * cut.Cg + i % cut.Cg;
       const double d = (double)smean[q] - mean;
       if (scnt[q] > 0.f) m2 += (double)sm2[q] + (double)scnt[q] * d * d;
     }
-    m2 = wave_sum_d(m2);
-    if (lane == 0) {
+    m2 = team_sum(m2, cut.team);
+    if (mine && lane == 0) {
       double* o = part + ((long)blockIdx.x * cut.G + g) * 3;
       o[0] = n;
       o[1] = mean;
@@ -241,60 +286,104 @@ __global__ __launch_bounds__(64) void gn_stats_join_kernel(const double* __restr
 }
 
 // ---------------------------------------------------------------------------------------------------- forward map
+// (The chunks are taken in reverse order: what the statistics pass read last is still in the cache.)
 template <typename T, int ACT>
 __global__ __launch_bounds__(1024) void gn_apply_kernel(const T* __restrict__ x, const float* __restrict__ gamma,
                                                         const float* __restrict__ beta,
                                                         const double* __restrict__ stats, T* __restrict__ y,
                                                         const Cut cut) {
-  constexpr int V = Io<T>::V;
+  constexpr int V = Io<T>::V, U = 4;
   const int tid = threadIdx.x;
-  const long b = blockIdx.x / cut.nchunk, ch = blockIdx.x % cut.nchunk;
-  const T* xs = x + b * cut.S;
-  T* ys = y + b * cut.S;
+  const long blk = (long)gridDim.x - 1 - blockIdx.x, b = blk / cut.nchunk, ch = blk % cut.nchunk;
   for (int col = 0; col < cut.columns; ++col) {
     const int t = col * cut.active + tid;
     if (tid >= cut.active || t >= cut.row) continue;
-    float mean[V], a[V], o[V];
+    const Share me = share_of<V>(cut, ch, t);
+    if (me.full + me.rest == 0) continue;
+    const T* p = x + b * cut.S + me.at;
+    T* o = y + b * cut.S + me.at;
+    const long hop = (long)cut.row * V;
+    float mean[V], a[V], c0[V];
+    int c = (int)(((long)t * V) % cut.C);
 #pragma unroll
     for (int e = 0; e < V; ++e) {
-      const int c = (int)(((long)t * V + e) % cut.C);
       const double* st = stats + 2 * (b * cut.G + c / cut.Cg);
       mean[e] = (float)st[0];
       a[e] = (float)st[1] * (gamma ? gamma[c] : 1.f);
-      o[e] = beta ? beta[c] : 0.f;
+      c0[e] = beta ? beta[c] : 0.f;
+      if (++c == cut.C) c = 0;
     }
-    const long v0 = ch * cut.iters * (long)cut.row + t;
-    for (int it = 0; it < cut.iters; ++it) {
-      const long v = v0 + it * (long)cut.row;
-      if (v >= cut.nvec) break;
-      const long at = v * V;
-      float f[V];
-      if (at + V <= cut.S) {
-        Io<T>::load(xs + at, f);
+    auto map = [&](Pack<T, V>& f) {
+      float v[V];
+      f.get(v);
 #pragma unroll
-        for (int e = 0; e < V; ++e) f[e] = act_fwd<ACT>(fmaf(f[e] - mean[e], a[e], o[e]));
-        Io<T>::store(ys + at, f);
-      } else {
-        for (int e = 0; e < (int)(cut.S - at); ++e)
-          ys[at + e] = Io<T>::from(act_fwd<ACT>(fmaf(Io<T>::to(xs[at + e]) - mean[e], a[e], o[e])));
+      for (int e = 0; e < V; ++e) v[e] = act_fwd<ACT>(fmaf(v[e] - mean[e], a[e], c0[e]));
+      f.set(v);
+    };
+    int it = 0;
+    for (; it + U <= me.full; it += U, p += U * hop, o += U * hop) {
+      Pack<T, V> f[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) f[u].load(p + u * hop);
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        map(f[u]);
+        f[u].store(o + u * hop);
       }
     }
+    for (; it < me.full; ++it, p += hop, o += hop) {
+      Pack<T, V> f;
+      f.load(p);
+      map(f);
+      f.store(o);
+    }
+#pragma unroll
+    for (int e = 0; e < V; ++e)
+      if (e < me.rest) o[e] = Io<T>::from(act_fwd<ACT>(fmaf(Io<T>::to(p[e]) - mean[e], a[e], c0[e])));
   }
 }
 
 // ---------------------------------------------------------------------------------------------------- backward
-// The slope of the activation at z.  Which side of zero a ReLU's input lies on decides a whole gradient element, so
-// where the 32-bit z is within its own rounding of zero the decision is made in 64 bits from the 64-bit statistics.
-template <int ACT>
-__device__ __forceinline__ float gn_slope(float x, float xh, float gam, float bet, const double* __restrict__ st) {
-  const float z = fmaf(xh, gam, bet);
-  if (ACT == ACT_RELU) {
-    const float mr = fabsf((float)(st[0] * st[1]));
-    if (fabsf(z) <= 3.8e-6f * (fabsf(gam) * (fabsf(xh) + mr) + fabsf(bet)))
-      return ((double)x - st[0]) * st[1] * (double)gam + (double)bet > 0.0 ? 1.f : 0.f;
+// what a thread knows of the channels of its V values: z = (x - mean) a + beta with a = gamma rstd
+template <int V>
+struct Channel {
+  float mean[V], a[V], bet[V];
+  int c, C, Cg;
+  const float* gamma;
+  const double* stats;      // of the sample
+  __device__ __forceinline__ void load(const double* st, const float* gam, const float* beta, int first, int channels,
+                                       int per_group) {
+    c = first;
+    C = channels;
+    Cg = per_group;
+    gamma = gam;
+    stats = st;
+    int k = first;
+#pragma unroll
+    for (int e = 0; e < V; ++e) {
+      mean[e] = (float)st[2 * (k / Cg)];
+      a[e] = (float)st[2 * (k / Cg) + 1] * (gam ? gam[k] : 1.f);
+      bet[e] = beta ? beta[k] : 0.f;
+      if (++k == C) k = 0;
+    }
   }
-  return act_slope<ACT>(z);
-}
+  // d = x - mean and the slope of the activation there.  Which side of zero a ReLU's input lies on decides a whole
+  // gradient element, so where the 32-bit z is within its own rounding of zero the decision is made in 64 bits from the
+  // 64-bit statistics.
+  template <int ACT>
+  __device__ __forceinline__ float slope(int e, float x, float& d) const {
+    d = x - mean[e];
+    const float z = fmaf(d, a[e], bet[e]);
+    if (ACT == ACT_RELU) {
+      if (fabsf(z) <= 3.8e-6f * (fabsf(a[e]) * (fabsf(d) + fabsf(mean[e])) + fabsf(bet[e]))) {
+        const int k = (c + e) % C;
+        const double* st = stats + 2 * (k / Cg);
+        return ((double)x - st[0]) * st[1] * (gamma ? (double)gamma[k] : 1.0) + (double)bet[e] > 0.0 ? 1.f : 0.f;
+      }
+    }
+    return act_slope<ACT>(z);
+  }
+};
 
 // per chunk and channel: sum of dz and of dz xhat
 template <typename T, int ACT>
@@ -303,54 +392,56 @@ __global__ __launch_bounds__(1024) void gn_bwd_sums_kernel(const T* __restrict__
                                                            const float* __restrict__ beta,
                                                            const double* __restrict__ stats, const Cut cut,
                                                            float* __restrict__ part) {
-  constexpr int V = Io<T>::V;
+  constexpr int V = Io<T>::V, U = 2;
   extern __shared__ float sh[];
   const int tid = threadIdx.x;
   const long b = blockIdx.x / cut.nchunk, ch = blockIdx.x % cut.nchunk;
-  const T* xs = x + b * cut.S;
-  const T* gs = dy + b * cut.S;
   const int slots = cut.columns == 1 ? cut.active * V : cut.period * V;
   for (int col = 0; col < cut.columns; ++col) {
     const int t = col * cut.active + tid;
     if (tid >= cut.active || t >= cut.row) continue;
-    float mean[V], rstd[V], gam[V], bet[V], s1[V], s2[V];
-    const double* st[V];
+    const Share me = share_of<V>(cut, ch, t);
+    const T* p = x + b * cut.S + me.at;
+    const T* g = dy + b * cut.S + me.at;
+    const long hop = (long)cut.row * V;
+    Channel<V> k;
+    k.load(stats + 2 * b * cut.G, gamma, beta, (int)(((long)t * V) % cut.C), cut.C, cut.Cg);
+    float s1[V], s2[V];           // sums of dz and of dz (x - mean)
 #pragma unroll
-    for (int e = 0; e < V; ++e) {
-      const int c = (int)(((long)t * V + e) % cut.C);
-      st[e] = stats + 2 * (b * cut.G + c / cut.Cg);
-      mean[e] = (float)st[e][0];
-      rstd[e] = (float)st[e][1];
-      gam[e] = gamma ? gamma[c] : 1.f;
-      bet[e] = beta ? beta[c] : 0.f;
-      s1[e] = s2[e] = 0.f;
-    }
-    const long v0 = ch * cut.iters * (long)cut.row + t;
-    for (int it = 0; it < cut.iters; ++it) {
-      const long v = v0 + it * (long)cut.row;
-      if (v >= cut.nvec) break;
-      const long at = v * V;
-      float f[V], d[V];
-      if (at + V <= cut.S) {
-        Io<T>::load(xs + at, f);
-        Io<T>::load(gs + at, d);
-      } else {
-        for (int e = 0; e < V; ++e) {
-          const bool in = at + e < cut.S;
-          f[e] = in ? Io<T>::to(xs[at + e]) : 0.f;
-          d[e] = in ? Io<T>::to(gs[at + e]) : 0.f;
-        }
-      }
+    for (int e = 0; e < V; ++e) s1[e] = s2[e] = 0.f;
+    auto add = [&](int e, float v, float h) {
+      float d;
+      const float dz = h * k.template slope<ACT>(e, v, d);
+      s1[e] += dz;
+      s2[e] = fmaf(dz, d, s2[e]);
+    };
+    int it = 0;
+    for (; it + U <= me.full; it += U, p += U * hop, g += U * hop) {
+      Pack<T, V> f[U], h[U];
 #pragma unroll
-      for (int e = 0; e < V; ++e) {
-        const float xh = (f[e] - mean[e]) * rstd[e];
-        const float dz = d[e] * gn_slope<ACT>(f[e], xh, gam[e], bet[e], st[e]);
-        s1[e] += dz;
-        s2[e] = fmaf(dz, xh, s2[e]);
+      for (int u = 0; u < U; ++u) f[u].load(p + u * hop), h[u].load(g + u * hop);
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        float v[V], d[V];
+        f[u].get(v);
+        h[u].get(d);
+#pragma unroll
+        for (int e = 0; e < V; ++e) add(e, v[e], d[e]);
       }
     }
+    for (; it < me.full; ++it, p += hop, g += hop) {
+      Pack<T, V> f, h;
+      f.load(p);
+      h.load(g);
+      float v[V], d[V];
+      f.get(v);
+      h.get(d);
+#pragma unroll
+      for (int e = 0; e < V; ++e) add(e, v[e], d[e]);
+    }
 #pragma unroll
     for (int e = 0; e < V; ++e) {
+      if (e < me.rest) add(e, Io<T>::to(p[e]), Io<T>::to(g[e]));
       sh[t * V + e] = s1[e];
       sh[slots + t * V + e] = s2[e];
     }
@@ -364,7 +455,7 @@ __global__ __launch_bounds__(1024) void gn_bwd_sums_kernel(const T* __restrict__
     }
     float* o = part + ((long)blockIdx.x * cut.C + c) * 2;
     o[0] = a;
-    o[1] = q;
+    o[1] = q * (float)stats[2 * (b * cut.G + c / cut.Cg) + 1];
   }
 }
 
@@ -413,7 +504,7 @@ __global__ __launch_bounds__(1024) void gn_bwd_apply_kernel(const T* __restrict_
                                                             const float* __restrict__ coef, T* __restrict__ dx,
                                                             float* __restrict__ dgamma, float* __restrict__ dbeta,
                                                             int nparam, long batch, const Cut cut) {
-  constexpr int V = Io<T>::V;
+  constexpr int V = Io<T>::V, U = 2;
   const int tid = threadIdx.x;
   if ((int)blockIdx.x < nparam) {
     const int c = blockIdx.x * blockDim.x + tid;
@@ -427,57 +518,65 @@ __global__ __launch_bounds__(1024) void gn_bwd_apply_kernel(const T* __restrict_
     if (dgamma) dgamma[c] = (float)q;
     return;
   }
-  const long blk = (long)blockIdx.x - nparam;
+  const long blk = (long)gridDim.x - 1 - blockIdx.x;      // in reverse order, as in the forward pass
   const long b = blk / cut.nchunk, ch = blk % cut.nchunk;
-  const T* xs = x + b * cut.S;
-  const T* gs = dy + b * cut.S;
-  T* os = dx + b * cut.S;
   for (int col = 0; col < cut.columns; ++col) {
     const int t = col * cut.active + tid;
     if (tid >= cut.active || t >= cut.row) continue;
-    float mean[V], rstd[V], gam[V], bet[V], k1[V], k2[V];
-    const double* st[V];
+    const Share me = share_of<V>(cut, ch, t);
+    if (me.full + me.rest == 0) continue;
+    const T* p = x + b * cut.S + me.at;
+    const T* g = dy + b * cut.S + me.at;
+    T* o = dx + b * cut.S + me.at;
+    const long hop = (long)cut.row * V;
+    Channel<V> k;
+    int c = (int)(((long)t * V) % cut.C);
+    k.load(stats + 2 * b * cut.G, gamma, beta, c, cut.C, cut.Cg);
+    float k1[V], k2[V];           // dx = a dz - k1 - (x - mean) k2
 #pragma unroll
     for (int e = 0; e < V; ++e) {
-      const int c = (int)(((long)t * V + e) % cut.C);
       const long bg = b * cut.G + c / cut.Cg;
-      st[e] = stats + 2 * bg;
-      mean[e] = (float)st[e][0];
-      rstd[e] = (float)st[e][1];
-      gam[e] = gamma ? gamma[c] : 1.f;
-      bet[e] = beta ? beta[c] : 0.f;
-      k1[e] = coef[2 * bg];
-      k2[e] = coef[2 * bg + 1];
+      const float rstd = (float)stats[2 * bg + 1];
+      k1[e] = coef[2 * bg] * rstd;
+      k2[e] = coef[2 * bg + 1] * rstd * rstd;
+      if (++c == cut.C) c = 0;
     }
-    const long v0 = ch * cut.iters * (long)cut.row + t;
-    for (int it = 0; it < cut.iters; ++it) {
-      const long v = v0 + it * (long)cut.row;
-      if (v >= cut.nvec) break;
-      const long at = v * V;
-      const bool whole = at + V <= cut.S;
-      float f[V], d[V];
-      if (whole) {
-        Io<T>::load(xs + at, f);
-        Io<T>::load(gs + at, d);
-      } else {
-        for (int e = 0; e < V; ++e) {
-          const bool in = at + e < cut.S;
-          f[e] = in ? Io<T>::to(xs[at + e]) : 0.f;
-          d[e] = in ? Io<T>::to(gs[at + e]) : 0.f;
-        }
-      }
+    auto value = [&](int e, float v, float h) {
+      float d;
+      const float dz = h * k.template slope<ACT>(e, v, d);
+      return fmaf(k.a[e], dz, -fmaf(d, k2[e], k1[e]));
+    };
+    int it = 0;
+    for (; it + U <= me.full; it += U, p += U * hop, g += U * hop, o += U * hop) {
+      Pack<T, V> f[U], h[U];
 #pragma unroll
-      for (int e = 0; e < V; ++e) {
-        const float xh = (f[e] - mean[e]) * rstd[e];
-        const float q = d[e] * gn_slope<ACT>(f[e], xh, gam[e], bet[e], st[e]) * gam[e];
-        f[e] = rstd[e] * (q - fmaf(xh, k2[e], k1[e]));
-      }
-      if (whole) {
-        Io<T>::store(os + at, f);
-      } else {
-        for (int e = 0; e < (int)(cut.S - at); ++e) os[at + e] = Io<T>::from(f[e]);
+      for (int u = 0; u < U; ++u) f[u].load(p + u * hop), h[u].load(g + u * hop);
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        float v[V], d[V];
+        f[u].get(v);
+        h[u].get(d);
+#pragma unroll
+        for (int e = 0; e < V; ++e) v[e] = value(e, v[e], d[e]);
+        f[u].set(v);
+        f[u].store(o + u * hop);
       }
     }
+    for (; it < me.full; ++it, p += hop, g += hop, o += hop) {
+      Pack<T, V> f, h;
+      f.load(p);
+      h.load(g);
+      float v[V], d[V];
+      f.get(v);
+      h.get(d);
+#pragma unroll
+      for (int e = 0; e < V; ++e) v[e] = value(e, v[e], d[e]);
+      f.set(v);
+      f.store(o);
+    }
+#pragma unroll
+    for (int e = 0; e < V; ++e)
+      if (e < me.rest) o[e] = Io<T>::from(value(e, Io<T>::to(p[e]), Io<T>::to(g[e])));
   }
 }
 
@@ -516,12 +615,16 @@ bool make_cut(long batch, long positions, int C, int G, int dtype, Cut* cut) {
     cut->row = cut->period;
   }
   const long rows = (cut->nvec + cut->row - 1) / cut->row;
-  // chunks: about eight blocks for every compute unit over the whole batch, at least four rows each
-  long iters = (rows * batch + 2047) / 2048;
-  if (iters < 4) iters = 4;
+  // chunks: about four blocks of 256 threads for every compute unit over the whole batch, at least eight rows each (a
+  // block's prologue and the joining of its sums cost about as much as four)
+  long iters = (rows * batch + 1023) / 1024;
+  if (iters < 8) iters = 8;
   if (iters > rows) iters = rows;
   cut->iters = (int)iters;
   cut->nchunk = (rows + iters - 1) / iters;
+  const int threads = (cut->active + 63) / 64 * 64;
+  cut->team = 64;
+  while (cut->team > 1 && threads / cut->team < G) cut->team >>= 1;
   return true;
 }
 

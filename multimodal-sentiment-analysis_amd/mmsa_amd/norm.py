@@ -16,29 +16,44 @@ from torch.autograd.function import once_differentiable
 from . import _lib, ops
 
 
+def _rows(x: torch.Tensor) -> torch.Tensor:
+    """[B, C, *positions] -> contiguous [B, P, C]; no copy for a map in channels-last memory."""
+    B, C = x.shape[:2]
+    if x.dim() == 4:
+        return x.permute(0, 2, 3, 1).contiguous().view(B, x.shape[2] * x.shape[3], C)
+    return x.movedim(1, -1).contiguous().view(B, math.prod(x.shape[2:]), C)
+
+
+def _maps(rows: torch.Tensor, shape) -> torch.Tensor:
+    """[B, P, C] -> [B, C, *positions] in channels-last memory."""
+    if len(shape) == 4:
+        return rows.view(shape[0], shape[2], shape[3], shape[1]).permute(0, 3, 1, 2)
+    return rows.view(shape[0], *shape[2:], shape[1]).movedim(-1, 1)
+
+
 class _GroupNormActFn(torch.autograd.Function):
-    """x [B, P, C] contiguous -> y [B, P, C]."""
+    """One node from the map as the caller holds it to the result: the changes of layout are views made inside it."""
 
     @staticmethod
     def forward(ctx, x, weight, bias, groups, eps, act):
-        y = torch.empty_like(x)
-        stats = torch.empty((x.shape[0], groups, 2), dtype=torch.float64, device=x.device)
-        ops.group_norm_act_fwd(x, weight, bias, y, stats, groups, eps, act)
-        ctx.save_for_backward(x, weight, bias, stats)
-        ctx.groups, ctx.act = groups, act
-        return y
+        rows = _rows(x)
+        y = torch.empty_like(rows)
+        stats = torch.empty((rows.shape[0], groups, 2), dtype=torch.float64, device=x.device)
+        ops.group_norm_act_fwd(rows, weight, bias, y, stats, groups, eps, act)
+        ctx.save_for_backward(rows, weight, bias, stats)
+        ctx.groups, ctx.act, ctx.shape = groups, act, x.shape
+        return _maps(y, x.shape)
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
-        x, weight, bias, stats = ctx.saved_tensors
+        rows, weight, bias, stats = ctx.saved_tensors
         want = ctx.needs_input_grad
-        with torch.cuda.device(x.device):
-            dx = torch.empty_like(x) if want[0] else None
-            dw = torch.empty_like(weight) if weight is not None and want[1] else None
-            db = torch.empty_like(bias) if bias is not None and want[2] else None
-            ops.group_norm_act_bwd(dy.contiguous(), x, weight, bias, stats, dx, dw, db, ctx.groups, ctx.act)
-        return dx, dw, db, None, None, None
+        dx = torch.empty_like(rows) if want[0] else None
+        dw = torch.empty_like(weight) if want[1] else None
+        db = torch.empty_like(bias) if want[2] else None
+        ops.group_norm_act_bwd(_rows(dy), rows, weight, bias, stats, dx, dw, db, ctx.groups, ctx.act)
+        return None if dx is None else _maps(dx, ctx.shape), dw, db, None, None, None
 
 
 def group_norm_act(x: torch.Tensor, num_groups: int, weight=None, bias=None, eps: float = 1e-5,
@@ -57,15 +72,14 @@ def group_norm_act(x: torch.Tensor, num_groups: int, weight=None, bias=None, eps
     B, C = x.shape[:2]
     if num_groups < 1 or C % num_groups or C < 1:
         raise ValueError(f"group_norm_act: {C} channels do not divide into {num_groups} groups")
-    rows = x.movedim(1, -1)
-    flat = rows.reshape(B, math.prod(x.shape[2:]), C).contiguous()
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias)):
-        y = _GroupNormActFn.apply(flat, weight, bias, num_groups, eps, activation)
-    else:
-        y = torch.empty_like(flat)
-        stats = torch.empty((B, num_groups, 2), dtype=torch.float64, device=x.device)
-        ops.group_norm_act_fwd(flat, weight, bias, y, stats, num_groups, eps, activation)
-    return y.view(rows.shape).movedim(-1, 1)
+    if torch.is_grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad)
+                                    or (bias is not None and bias.requires_grad)):
+        return _GroupNormActFn.apply(x, weight, bias, num_groups, eps, activation)
+    rows = _rows(x)
+    y = torch.empty_like(rows)
+    stats = torch.empty((B, num_groups, 2), dtype=torch.float64, device=x.device)
+    ops.group_norm_act_fwd(rows, weight, bias, y, stats, num_groups, eps, activation)
+    return _maps(y, x.shape)
 
 
 class GroupNormAct(nn.Module):
