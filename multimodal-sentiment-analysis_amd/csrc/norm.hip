@@ -55,6 +55,9 @@ template <> struct Bits<2> { typedef unsigned short type; };
 template <typename T, int W> struct Pack {
   typename Bits<W * (int)sizeof(T)>::type raw;
   __device__ __forceinline__ void load(const T* p) { raw = *reinterpret_cast<const decltype(raw)*>(p); }
+  __device__ __forceinline__ void load_once(const T* p) {
+    raw = __builtin_nontemporal_load(reinterpret_cast<const decltype(raw)*>(p));
+  }
   __device__ __forceinline__ void store(T* p) const { *reinterpret_cast<decltype(raw)*>(p) = raw; }
   __device__ __forceinline__ void get(float (&o)[W]) const {
     T v[W];
@@ -112,7 +115,7 @@ __device__ __forceinline__ float act_slope(float z) {
 }
 
 // How a sample is cut: `active` threads of a block cover rows of `active` vectors (a multiple of the period), `columns`
-// of them one after another where the period is longer than a block; a chunk is `iters` such rows.
+// of them one after another where the period is longer than a block; a chunk is at most `iters` such rows.
 struct Cut {
   long S;          // values per sample
   long nvec;       // vectors per sample, the last one possibly cut short
@@ -130,22 +133,23 @@ __device__ __forceinline__ double team_sum(double v, int team) {
   return v;
 }
 
-// a thread's share of a chunk: `full` whole vectors, `row` apart, from the first on; then possibly the sample's last,
-// shorter one
+// A thread's share of a chunk: `full` whole vectors, `hop` values apart, from the first on; then possibly the sample's
+// last, shorter one.  A chunk takes every nchunk-th row of threads, so that all blocks sweep through the sample together:
+// blocks that each stream a run of their own, a power of two apart, crowd on a few memory channels.
 struct Share {
-  long at;      // first value
+  long at, hop;
   int full;
   int rest;     // values of the short vector behind them, 0: none
 };
 template <int V>
 __device__ __forceinline__ Share share_of(const Cut& cut, long ch, int t) {
-  const long v0 = ch * cut.iters * (long)cut.row + t, whole = cut.S / V;
+  const long v0 = ch * cut.row + t, step = cut.nchunk * cut.row, whole = cut.S / V;
   Share s;
   s.at = v0 * V;
-  long n = v0 < whole ? (whole - v0 + cut.row - 1) / cut.row : 0;
-  if (n > cut.iters) n = cut.iters;
+  s.hop = step * V;
+  const long n = v0 < whole ? (whole - v0 + step - 1) / step : 0;
   s.full = (int)n;
-  s.rest = n < cut.iters && v0 + n * cut.row == whole ? (int)(cut.S - whole * V) : 0;
+  s.rest = v0 + n * step == whole ? (int)(cut.S - whole * V) : 0;
   return s;
 }
 
@@ -154,7 +158,9 @@ __device__ __forceinline__ Share share_of(const Cut& cut, long ch, int t) {
 // sum of squares about the thread's mean loses at most a few roundings to cancellation, whatever the mean of the map
 // is.  Threads, chunks and channels are then joined in 64 bits by the parallel-variance formula
 //   M2 = sum M2_i + sum n_i (mean_i - mean)^2.
-template <typename T>
+// ONCE: the map is larger than what the last-level cache would keep for the next pass; reading it past that cache spares
+// the eviction of dirty lines (268 MB: 52 us instead of 80).
+template <typename T, bool ONCE>
 __global__ __launch_bounds__(1024) void gn_stats_kernel(const T* __restrict__ x, const Cut cut,
                                                         double* __restrict__ part) {
   constexpr int V = Io<T>::V, U = 4;            // U loads in flight per thread
@@ -171,7 +177,7 @@ __global__ __launch_bounds__(1024) void gn_stats_kernel(const T* __restrict__ x,
     if (tid >= cut.active || t >= cut.row) continue;
     const Share me = share_of<V>(cut, ch, t);
     const T* p = xs + me.at;
-    const long hop = (long)cut.row * V;
+    const long hop = me.hop;
     float k[V], s[V], q[V];
 #pragma unroll
     for (int e = 0; e < V; ++e) k[e] = s[e] = q[e] = 0.f;
@@ -184,7 +190,12 @@ __global__ __launch_bounds__(1024) void gn_stats_kernel(const T* __restrict__ x,
     for (; it + U <= me.full; it += U, p += U * hop) {
       Pack<T, V> f[U];
 #pragma unroll
-      for (int u = 0; u < U; ++u) f[u].load(p + u * hop);
+      for (int u = 0; u < U; ++u) {
+        if (ONCE)
+          f[u].load_once(p + u * hop);
+        else
+          f[u].load(p + u * hop);
+      }
 #pragma unroll
       for (int u = 0; u < U; ++u) {
         float v[V];
@@ -286,15 +297,14 @@ __global__ __launch_bounds__(64) void gn_stats_join_kernel(const double* __restr
 }
 
 // ---------------------------------------------------------------------------------------------------- forward map
-// (The chunks are taken in reverse order: what the statistics pass read last is still in the cache.)
-template <typename T, int ACT>
+template <typename T, int ACT, bool ONCE>
 __global__ __launch_bounds__(1024) void gn_apply_kernel(const T* __restrict__ x, const float* __restrict__ gamma,
                                                         const float* __restrict__ beta,
                                                         const double* __restrict__ stats, T* __restrict__ y,
                                                         const Cut cut) {
   constexpr int V = Io<T>::V, U = 4;
   const int tid = threadIdx.x;
-  const long blk = (long)gridDim.x - 1 - blockIdx.x, b = blk / cut.nchunk, ch = blk % cut.nchunk;
+  const long blk = (long)gridDim.x - 1 - blockIdx.x, b = blk / cut.nchunk, ch = blk % cut.nchunk;   // reversed too
   for (int col = 0; col < cut.columns; ++col) {
     const int t = col * cut.active + tid;
     if (tid >= cut.active || t >= cut.row) continue;
@@ -302,7 +312,7 @@ __global__ __launch_bounds__(1024) void gn_apply_kernel(const T* __restrict__ x,
     if (me.full + me.rest == 0) continue;
     const T* p = x + b * cut.S + me.at;
     T* o = y + b * cut.S + me.at;
-    const long hop = (long)cut.row * V;
+    const long hop = me.hop;
     float mean[V], a[V], c0[V];
     int c = (int)(((long)t * V) % cut.C);
 #pragma unroll
@@ -313,6 +323,12 @@ __global__ __launch_bounds__(1024) void gn_apply_kernel(const T* __restrict__ x,
       c0[e] = beta ? beta[c] : 0.f;
       if (++c == cut.C) c = 0;
     }
+    // backwards: what the statistics pass read last is still in the cache
+    p += me.full * hop;
+    o += me.full * hop;
+#pragma unroll
+    for (int e = 0; e < V; ++e)
+      if (e < me.rest) o[e] = Io<T>::from(act_fwd<ACT>(fmaf(Io<T>::to(p[e]) - mean[e], a[e], c0[e])));
     auto map = [&](Pack<T, V>& f) {
       float v[V];
       f.get(v);
@@ -320,26 +336,32 @@ __global__ __launch_bounds__(1024) void gn_apply_kernel(const T* __restrict__ x,
       for (int e = 0; e < V; ++e) v[e] = act_fwd<ACT>(fmaf(v[e] - mean[e], a[e], c0[e]));
       f.set(v);
     };
-    int it = 0;
-    for (; it + U <= me.full; it += U, p += U * hop, o += U * hop) {
+    int it = me.full;
+    for (; it >= U; it -= U) {
+      p -= U * hop;
+      o -= U * hop;
       Pack<T, V> f[U];
 #pragma unroll
-      for (int u = 0; u < U; ++u) f[u].load(p + u * hop);
+      for (int u = 0; u < U; ++u) {
+        if (ONCE)
+          f[u].load_once(p + u * hop);
+        else
+          f[u].load(p + u * hop);
+      }
 #pragma unroll
       for (int u = 0; u < U; ++u) {
         map(f[u]);
         f[u].store(o + u * hop);
       }
     }
-    for (; it < me.full; ++it, p += hop, o += hop) {
+    for (; it > 0; --it) {
+      p -= hop;
+      o -= hop;
       Pack<T, V> f;
       f.load(p);
       map(f);
       f.store(o);
     }
-#pragma unroll
-    for (int e = 0; e < V; ++e)
-      if (e < me.rest) o[e] = Io<T>::from(act_fwd<ACT>(fmaf(Io<T>::to(p[e]) - mean[e], a[e], c0[e])));
   }
 }
 
@@ -386,7 +408,7 @@ struct Channel {
 };
 
 // per chunk and channel: sum of dz and of dz xhat
-template <typename T, int ACT>
+template <typename T, int ACT, bool ONCE>
 __global__ __launch_bounds__(1024) void gn_bwd_sums_kernel(const T* __restrict__ dy, const T* __restrict__ x,
                                                            const float* __restrict__ gamma,
                                                            const float* __restrict__ beta,
@@ -403,7 +425,7 @@ __global__ __launch_bounds__(1024) void gn_bwd_sums_kernel(const T* __restrict__
     const Share me = share_of<V>(cut, ch, t);
     const T* p = x + b * cut.S + me.at;
     const T* g = dy + b * cut.S + me.at;
-    const long hop = (long)cut.row * V;
+    const long hop = me.hop;
     Channel<V> k;
     k.load(stats + 2 * b * cut.G, gamma, beta, (int)(((long)t * V) % cut.C), cut.C, cut.Cg);
     float s1[V], s2[V];           // sums of dz and of dz (x - mean)
@@ -419,7 +441,12 @@ __global__ __launch_bounds__(1024) void gn_bwd_sums_kernel(const T* __restrict__
     for (; it + U <= me.full; it += U, p += U * hop, g += U * hop) {
       Pack<T, V> f[U], h[U];
 #pragma unroll
-      for (int u = 0; u < U; ++u) f[u].load(p + u * hop), h[u].load(g + u * hop);
+      for (int u = 0; u < U; ++u) {
+        if (ONCE)
+          f[u].load_once(p + u * hop), h[u].load_once(g + u * hop);
+        else
+          f[u].load(p + u * hop), h[u].load(g + u * hop);
+      }
 #pragma unroll
       for (int u = 0; u < U; ++u) {
         float v[V], d[V];
@@ -494,8 +521,37 @@ __global__ __launch_bounds__(256) void gn_bwd_join_kernel(const float* __restric
   }
 }
 
-// blocks [0, nparam): dgamma / dbeta, a channel per thread, summed over the samples in order; the others: dx
-template <typename T, int ACT>
+// dgamma / dbeta of 64 channels: a channel per lane, the samples shared out among the block's waves, joined in order
+__device__ __forceinline__ void param_sums(const float* __restrict__ sums, long batch, int C, int c0,
+                                           float* __restrict__ dgamma, float* __restrict__ dbeta, double (*red)[64][2]) {
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, nw = blockDim.x >> 6, c = c0 + lane;
+  double a = 0.0, q = 0.0;
+  if (c < C) {
+#pragma unroll 4
+    for (long b = w; b < batch; b += nw) {
+      a += (double)sums[(b * C + c) * 2];
+      q += (double)sums[(b * C + c) * 2 + 1];
+    }
+  }
+  red[w][lane][0] = a;
+  red[w][lane][1] = q;
+  __syncthreads();
+  if (w || c >= C) return;
+  for (int k = 1; k < nw; ++k) {
+    a += red[k][lane][0];
+    q += red[k][lane][1];
+  }
+  if (dbeta) dbeta[c] = (float)a;
+  if (dgamma) dgamma[c] = (float)q;
+}
+__global__ __launch_bounds__(1024) void gn_param_kernel(const float* __restrict__ sums, long batch, int C,
+                                                        float* __restrict__ dgamma, float* __restrict__ dbeta) {
+  __shared__ double red[16][64][2];
+  param_sums(sums, batch, C, blockIdx.x * 64, dgamma, dbeta, red);
+}
+
+// blocks [0, nparam): dgamma / dbeta; the others: dx
+template <typename T, int ACT, bool ONCE>
 __global__ __launch_bounds__(1024) void gn_bwd_apply_kernel(const T* __restrict__ dy, const T* __restrict__ x,
                                                             const float* __restrict__ gamma,
                                                             const float* __restrict__ beta,
@@ -507,18 +563,11 @@ __global__ __launch_bounds__(1024) void gn_bwd_apply_kernel(const T* __restrict_
   constexpr int V = Io<T>::V, U = 2;
   const int tid = threadIdx.x;
   if ((int)blockIdx.x < nparam) {
-    const int c = blockIdx.x * blockDim.x + tid;
-    if (c >= cut.C) return;
-    double a = 0.0, q = 0.0;
-    for (long b = 0; b < batch; ++b) {
-      a += (double)sums[(b * cut.C + c) * 2];
-      q += (double)sums[(b * cut.C + c) * 2 + 1];
-    }
-    if (dbeta) dbeta[c] = (float)a;
-    if (dgamma) dgamma[c] = (float)q;
+    __shared__ double red[16][64][2];
+    param_sums(sums, batch, cut.C, blockIdx.x * 64, dgamma, dbeta, red);
     return;
   }
-  const long blk = (long)gridDim.x - 1 - blockIdx.x;      // in reverse order, as in the forward pass
+  const long blk = (long)gridDim.x - 1 - blockIdx.x;      // the samples in reverse order too
   const long b = blk / cut.nchunk, ch = blk % cut.nchunk;
   for (int col = 0; col < cut.columns; ++col) {
     const int t = col * cut.active + tid;
@@ -528,7 +577,7 @@ __global__ __launch_bounds__(1024) void gn_bwd_apply_kernel(const T* __restrict_
     const T* p = x + b * cut.S + me.at;
     const T* g = dy + b * cut.S + me.at;
     T* o = dx + b * cut.S + me.at;
-    const long hop = (long)cut.row * V;
+    const long hop = me.hop;
     Channel<V> k;
     int c = (int)(((long)t * V) % cut.C);
     k.load(stats + 2 * b * cut.G, gamma, beta, c, cut.C, cut.Cg);
@@ -546,11 +595,25 @@ __global__ __launch_bounds__(1024) void gn_bwd_apply_kernel(const T* __restrict_
       const float dz = h * k.template slope<ACT>(e, v, d);
       return fmaf(k.a[e], dz, -fmaf(d, k2[e], k1[e]));
     };
-    int it = 0;
-    for (; it + U <= me.full; it += U, p += U * hop, g += U * hop, o += U * hop) {
+    p += me.full * hop;           // backwards, as in the forward pass
+    g += me.full * hop;
+    o += me.full * hop;
+#pragma unroll
+    for (int e = 0; e < V; ++e)
+      if (e < me.rest) o[e] = Io<T>::from(value(e, Io<T>::to(p[e]), Io<T>::to(g[e])));
+    int it = me.full;
+    for (; it >= U; it -= U) {
+      p -= U * hop;
+      g -= U * hop;
+      o -= U * hop;
       Pack<T, V> f[U], h[U];
 #pragma unroll
-      for (int u = 0; u < U; ++u) f[u].load(p + u * hop), h[u].load(g + u * hop);
+      for (int u = 0; u < U; ++u) {
+        if (ONCE)
+          f[u].load_once(p + u * hop), h[u].load_once(g + u * hop);
+        else
+          f[u].load(p + u * hop), h[u].load(g + u * hop);
+      }
 #pragma unroll
       for (int u = 0; u < U; ++u) {
         float v[V], d[V];
@@ -562,7 +625,10 @@ __global__ __launch_bounds__(1024) void gn_bwd_apply_kernel(const T* __restrict_
         f[u].store(o + u * hop);
       }
     }
-    for (; it < me.full; ++it, p += hop, g += hop, o += hop) {
+    for (; it > 0; --it) {
+      p -= hop;
+      g -= hop;
+      o -= hop;
       Pack<T, V> f, h;
       f.load(p);
       h.load(g);
@@ -574,9 +640,311 @@ __global__ __launch_bounds__(1024) void gn_bwd_apply_kernel(const T* __restrict_
       f.set(v);
       f.store(o);
     }
+  }
+}
+
+// ------------------------------------------------------------------------------------- groups that fit one block
+// A block keeps its slab -- the P positions of `bundle` groups of one sample -- in registers: one read, one launch, no
+// partial sums.  Thread t always has the same W channels (column t % nw of a row of the slab) and every rp-th row.  The
+// statistics take two passes over the registers, the second one correcting the mean of the first:
+//   m = sum x / N,  d = x - m,  mean = m + sum d / N,  var = (sum d^2 - (sum d)^2 / N) / N,
+// exact to rounding whatever the mean is.  A bundle has at least 64 bytes of a row where enough blocks remain; the
+// bundles of one sample run on one XCD, whose L2 they share.
+struct Slab {
+  long S;          // values per sample
+  int P, C, G, Cg;
+  int W;           // values per vector, divides Cg
+  int bundle;      // groups per block
+  int bundles;     // blocks per sample
+  int nw, rp;      // vectors in a row of the slab, rows per pass of the block
+  int threads, vecs;
+  long batch;
+};
+struct Place {
+  long b;
+  int c0, L, nw, G;     // first channel, channels, vectors a row, groups
+};
+__device__ __forceinline__ Place place_of(const Slab& q) {
+  // eight samples side by side, one per XCD
+  const long l = blockIdx.x, per = 8l * q.bundles, eights = q.batch >> 3;
+  Place p;
+  long k;
+  if (l < eights * per) {
+    p.b = l / per * 8 + (l & 7);
+    k = l % per >> 3;
+  } else {
+    const long r = l - eights * per;
+    p.b = eights * 8 + r / q.bundles;
+    k = r % q.bundles;
+  }
+  const int g0 = (int)k * q.bundle;
+  p.G = q.G - g0 < q.bundle ? q.G - g0 : q.bundle;
+  p.c0 = g0 * q.Cg;
+  p.L = p.G * q.Cg;
+  p.nw = p.L / q.W;
+  return p;
+}
+
+// sums over the groups of two values per thread; `out` holds them for every group afterwards
+__device__ __forceinline__ void group_sums(float a, float b, const Slab& q, const Place& p, float2* red,
+                                           double (*out)[2]) {
+  const int tid = threadIdx.x, cw = q.Cg / q.W, per = q.rp * cw;
+  if (p.G == 1) {                               // uniform: the whole block is one group
+    const double s = wave_sum_d((double)a), t = wave_sum_d((double)b);
+    double2* part = reinterpret_cast<double2*>(red);
+    __syncthreads();
+    if ((tid & 63) == 0) part[tid >> 6] = make_double2(s, t);
+    __syncthreads();
+    double2 all = make_double2(0.0, 0.0);
+    for (int k = 0; k < (int)blockDim.x >> 6; ++k) all.x += part[k].x, all.y += part[k].y;
+    if (tid == 0) out[0][0] = all.x, out[0][1] = all.y;
+    __syncthreads();
+    return;
+  }
+  __syncthreads();
+  red[tid] = make_float2(a, b);
+  __syncthreads();
+  int team = 64;
+  while (team > 1 && (int)blockDim.x / team < p.G) team >>= 1;
+  const int lane = tid & (team - 1), teams = blockDim.x / team;
+  for (int g0 = 0; g0 < p.G; g0 += teams) {
+    const int g = g0 + tid / team;
+    double s = 0.0, t = 0.0;
+    for (int i = lane; g < p.G && i < per; i += team) {
+      const float2 v = red[(i / cw) * q.nw + g * cw + i % cw];
+      s += (double)v.x;
+      t += (double)v.y;
+    }
+    s = team_sum(s, team);
+    t = team_sum(t, team);
+    if (g < p.G && lane == 0) {
+      out[g][0] = s;
+      out[g][1] = t;
+    }
+  }
+  __syncthreads();
+}
+
+template <typename T, int W, int NV, int ACT>
+__device__ __forceinline__ void slab_store(Pack<T, W> (&f)[NV], const float (&mean)[W], const float (&a)[W],
+                                           const float (&bet)[W], T* y, int r0, const Slab& q) {
 #pragma unroll
-    for (int e = 0; e < V; ++e)
-      if (e < me.rest) o[e] = Io<T>::from(value(e, Io<T>::to(p[e]), Io<T>::to(g[e])));
+  for (int k = 0; k < NV; ++k) {
+    const int r = r0 + k * q.rp;
+    if (r < q.P) {
+      float v[W];
+      f[k].get(v);
+#pragma unroll
+      for (int e = 0; e < W; ++e) v[e] = act_fwd<ACT>(fmaf(v[e] - mean[e], a[e], bet[e]));
+      f[k].set(v);
+      f[k].store(y + (long)r * q.C);
+    }
+  }
+}
+
+constexpr int GN_MAX_BUNDLE = 64;
+
+template <typename T, int W, int NV>
+__global__ __launch_bounds__(1024) void gn_slab_fwd_kernel(const T* __restrict__ x, const float* __restrict__ gamma,
+                                                           const float* __restrict__ beta, T* __restrict__ y,
+                                                           double* __restrict__ stats, float eps, int act,
+                                                           const Slab q) {
+  __shared__ float2 red[1024];
+  __shared__ double sum[GN_MAX_BUNDLE][2];
+  const Place p = place_of(q);
+  const int tid = threadIdx.x, col = tid % q.nw, r0 = tid / q.nw;
+  const bool in = col < p.nw && r0 < q.rp;
+  const long at = p.b * q.S + p.c0 + col * W;
+  Pack<T, W> f[NV];
+  float s = 0.f;
+#pragma unroll
+  for (int k = 0; k < NV; ++k) {
+    const int r = r0 + k * q.rp;
+    if (in && r < q.P) f[k].load(x + at + (long)r * q.C);
+  }
+#pragma unroll
+  for (int k = 0; k < NV; ++k) {
+    if (in && r0 + k * q.rp < q.P) {
+      float v[W];
+      f[k].get(v);
+#pragma unroll
+      for (int e = 0; e < W; ++e) s += v[e];
+    }
+  }
+  float gam[W], bet[W];                         // asked for now, needed at the end
+#pragma unroll
+  for (int e = 0; e < W; ++e) {
+    const int c = in ? p.c0 + col * W + e : 0;
+    gam[e] = gamma ? gamma[c] : 1.f;
+    bet[e] = beta ? beta[c] : 0.f;
+  }
+  const int g = in ? col * W / q.Cg : 0;
+  const double n = (double)q.P * q.Cg;
+  group_sums(s, 0.f, q, p, red, sum);
+  const double m0 = sum[g][0] / n;
+  const float m = (float)m0;
+  float d1 = 0.f, d2 = 0.f;
+#pragma unroll
+  for (int k = 0; k < NV; ++k) {
+    if (in && r0 + k * q.rp < q.P) {
+      float v[W];
+      f[k].get(v);
+#pragma unroll
+      for (int e = 0; e < W; ++e) {
+        const float d = v[e] - m;
+        d1 += d;
+        d2 = fmaf(d, d, d2);
+      }
+    }
+  }
+  group_sums(d1, d2, q, p, red, sum);
+  const double off = sum[g][0] / n;
+  const double var = fmax(sum[g][1] / n - off * off, 0.0);
+  const double mean64 = (double)m + off;
+  // a NaN of the data passes fmax by: put it back
+  const double rstd64 = sum[g][1] == sum[g][1] ? 1.0 / sqrt(var + (double)eps) : sum[g][1];
+  if (in && r0 == 0 && col * W % q.Cg == 0) {
+    double* o = stats + 2 * (p.b * q.G + p.c0 / q.Cg + g);
+    o[0] = mean64;
+    o[1] = rstd64;
+  }
+  if (!in) return;
+  float mean[W], a[W];
+#pragma unroll
+  for (int e = 0; e < W; ++e) {
+    mean[e] = (float)mean64;
+    a[e] = (float)rstd64 * gam[e];
+  }
+  T* o = y + at;
+  switch (act) {
+    case ACT_NONE: slab_store<T, W, NV, ACT_NONE>(f, mean, a, bet, o, r0, q); break;
+    case ACT_RELU: slab_store<T, W, NV, ACT_RELU>(f, mean, a, bet, o, r0, q); break;
+    case ACT_SILU: slab_store<T, W, NV, ACT_SILU>(f, mean, a, bet, o, r0, q); break;
+    default: slab_store<T, W, NV, ACT_GELU>(f, mean, a, bet, o, r0, q); break;
+  }
+}
+
+// The backward pass of a slab: dx, and the sums of its channels for the parameter gradients.
+template <typename T, int W, int NV, int ACT>
+__global__ __launch_bounds__(1024) void gn_slab_bwd_kernel(const T* __restrict__ dy, const T* __restrict__ x,
+                                                           const float* __restrict__ gamma,
+                                                           const float* __restrict__ beta,
+                                                           const double* __restrict__ stats, T* __restrict__ dx,
+                                                           float* __restrict__ sums, const Slab q) {
+  extern __shared__ float sh[];                 // [rows][channels][2], then [segments][channels][2]
+  __shared__ double sum[GN_MAX_BUNDLE][2];
+  const Place p = place_of(q);
+  const int tid = threadIdx.x, col = tid % q.nw, r0 = tid / q.nw;
+  const bool in = col < p.nw && r0 < q.rp;
+  const long at = p.b * q.S + p.c0 + col * W;
+  const double* st = stats + 2 * p.b * q.G;
+  Pack<T, W> f[NV], h[NV];
+#pragma unroll
+  for (int k = 0; k < NV; ++k) {
+    const int r = r0 + k * q.rp;
+    if (in && r < q.P) {
+      f[k].load(x + at + (long)r * q.C);
+      h[k].load(dy + at + (long)r * q.C);
+    }
+  }
+  Channel<W> ch;
+  ch.load(st, gamma, beta, in ? p.c0 + col * W : p.c0, q.C, q.Cg);
+  float s1[W], s2[W];
+#pragma unroll
+  for (int e = 0; e < W; ++e) s1[e] = s2[e] = 0.f;
+#pragma unroll
+  for (int k = 0; k < NV; ++k) {
+    if (in && r0 + k * q.rp < q.P) {
+      float v[W], g[W];
+      f[k].get(v);
+      h[k].get(g);
+#pragma unroll
+      for (int e = 0; e < W; ++e) {
+        float d;
+        const float dz = g[e] * ch.template slope<ACT>(e, v[e], d);
+        s1[e] += dz;
+        s2[e] = fmaf(dz, d, s2[e]);
+      }
+    }
+  }
+  const int Lf = q.nw * W;                      // channels of a full bundle: the row pitch
+  float* seg = sh + 2 * q.rp * Lf;
+  if (r0 < q.rp) {
+#pragma unroll
+    for (int e = 0; e < W; ++e) {
+      sh[(r0 * Lf + col * W + e) * 2] = s1[e];
+      sh[(r0 * Lf + col * W + e) * 2 + 1] = s2[e];
+    }
+  }
+  __syncthreads();
+  const int nseg = (int)blockDim.x / p.L > 1 ? (int)blockDim.x / p.L : 1;
+  for (int i = tid; i < p.L * nseg; i += blockDim.x) {
+    const int c = i % p.L;
+    float a = 0.f, t = 0.f;
+    for (int r = i / p.L; r < q.rp; r += nseg) {
+      a += sh[(r * Lf + c) * 2];
+      t += sh[(r * Lf + c) * 2 + 1];
+    }
+    seg[2 * i] = a;
+    seg[2 * i + 1] = t;
+  }
+  __syncthreads();
+  for (int c = tid; c < p.L; c += blockDim.x) {
+    float a = 0.f, t = 0.f;
+    for (int i = c; i < p.L * nseg; i += p.L) {
+      a += seg[2 * i];
+      t += seg[2 * i + 1];
+    }
+    t *= (float)st[2 * ((p.c0 + c) / q.Cg) + 1];
+    float* o = sums + (p.b * q.C + p.c0 + c) * 2;
+    o[0] = a;
+    o[1] = t;
+    const float gm = gamma ? gamma[p.c0 + c] : 1.f;
+    sh[2 * c] = a * gm;
+    sh[2 * c + 1] = t * gm;
+  }
+  if (!dx) return;
+  __syncthreads();
+  int team = 64;
+  while (team > 1 && (int)blockDim.x / team < p.G) team >>= 1;
+  const int lane = tid & (team - 1), teams = blockDim.x / team;
+  for (int g0 = 0; g0 < p.G; g0 += teams) {
+    const int g = g0 + tid / team;
+    double a = 0.0, t = 0.0;
+    for (int i = lane; g < p.G && i < q.Cg; i += team) {
+      a += (double)sh[2 * (g * q.Cg + i)];
+      t += (double)sh[2 * (g * q.Cg + i) + 1];
+    }
+    a = team_sum(a, team);
+    t = team_sum(t, team);
+    if (g < p.G && lane == 0) {
+      sum[g][0] = a;
+      sum[g][1] = t;
+    }
+  }
+  __syncthreads();
+  if (!in) return;
+  const int g = col * W / q.Cg;
+  const double n = (double)q.P * q.Cg;
+  const float rstd = (float)st[2 * (p.c0 / q.Cg + g) + 1];
+  const float k1 = (float)(sum[g][0] / n) * rstd, k2 = (float)(sum[g][1] / n) * rstd * rstd;
+  T* o = dx + at;
+#pragma unroll
+  for (int k = 0; k < NV; ++k) {
+    const int r = r0 + k * q.rp;
+    if (r < q.P) {
+      float v[W], gr[W];
+      f[k].get(v);
+      h[k].get(gr);
+#pragma unroll
+      for (int e = 0; e < W; ++e) {
+        float d;
+        const float dz = gr[e] * ch.template slope<ACT>(e, v[e], d);
+        v[e] = fmaf(ch.a[e], dz, -fmaf(d, k2, k1));
+      }
+      f[k].set(v);
+      f[k].store(o + (long)r * q.C);
+    }
   }
 }
 
@@ -584,6 +952,7 @@ __global__ __launch_bounds__(1024) void gn_bwd_apply_kernel(const T* __restrict_
 constexpr int GN_MAX_CHANNELS = 4096;
 constexpr int GN_MAX_SLOTS = 12288;         // three floats of LDS for each: 144 of the 160 KiB
 constexpr long GN_MAX_BLOCKS = 4000000;     // a grid's threads are counted in 32 bits, blocks have up to 1024
+constexpr long GN_CACHED = 160l << 20;      // what a second pass still finds of the first one's reads in the 256 MB cache
 
 int value_lanes(int dtype) { return dtype == 0 ? 4 : 8; }
 
@@ -633,31 +1002,110 @@ size_t slots_of(const Cut& cut, int dtype) {
   return (size_t)(cut.columns == 1 ? cut.active : cut.period) * value_lanes(dtype);
 }
 // dynamic LDS of the sums kernels: a block's (thread, value) slots; at most 12 * GN_MAX_SLOTS bytes
-template <typename K>
-int allow_lds(K kernel, size_t bytes) {
+template <auto kernel>
+int allow_lds(size_t bytes) {
   static PerDeviceOnce once;
   if (bytes > 65536 && once.pending()) {
     if (hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize,
-                            160 * 1024) != hipSuccess)
+                            12 * GN_MAX_SLOTS) != hipSuccess)
       return MMSA_ERR_LAUNCH;
     once.done();
   }
   return MMSA_OK;
 }
 
-template <typename T>
-int gn_fwd(const void* x, const float* gamma, const float* beta, void* y, double* stats, void* scratch, long batch,
-           const Cut& cut, int dtype, float eps, int act, hipStream_t s) {
-  const T* xp = static_cast<const T*>(x);
-  T* yp = static_cast<T*>(y);
+// Whether a pass can keep its slabs in registers, and how.  `most`: registers of 4 bytes a thread may hold of one map.
+bool make_slab(long batch, long positions, int C, int G, int dtype, int most, Slab* q) {
+  const int size = dtype == 0 ? 4 : 2, Cg = C / G;
+  if (positions > 65536) return false;
+  q->S = positions * C;
+  q->P = (int)positions;
+  q->C = C;
+  q->G = G;
+  q->Cg = Cg;
+  q->batch = batch;
+  q->W = 1;
+  for (int w = 16 / size; w > 1; w >>= 1)
+    if (Cg % w == 0 && (w == 16 / size || size * w == 8)) {
+      q->W = w;
+      break;
+    }
+  const int reg = (q->W * size + 3) / 4;        // registers of a vector
+  int bundle = (64 + Cg * size - 1) / (Cg * size);
+  if (bundle > G) bundle = G;
+  if (batch * ((G + bundle - 1) / bundle) < 256) bundle = 1;
+  for (; bundle >= 1; bundle >>= 1) {
+    q->bundle = bundle;
+    q->bundles = (G + bundle - 1) / bundle;
+    q->nw = bundle * Cg / q->W;
+    for (int t = 256; t <= 1024; t <<= 1) {
+      if (q->nw > t) continue;
+      q->rp = t / q->nw;
+      q->threads = t;
+      q->vecs = (q->P + q->rp - 1) / q->rp;
+      const int cap = t < 1024 ? 4 : most / reg < 16 ? most / reg : 16;
+      if (q->vecs <= cap) return batch * q->bundles <= GN_MAX_BLOCKS;
+    }
+  }
+  return false;
+}
+
+template <typename T, int W, int NV>
+int slab_fwd(const void* x, const float* gamma, const float* beta, void* y, double* stats, float eps, int act,
+             const Slab& q, hipStream_t s) {
+  hipLaunchKernelGGL((gn_slab_fwd_kernel<T, W, NV>), dim3((unsigned)(q.batch * q.bundles)), dim3(q.threads), 0, s,
+                     static_cast<const T*>(x), gamma, beta, static_cast<T*>(y), stats, eps, act, q);
+  return mmsa_launch_status();
+}
+template <typename T, int W>
+int slab_fwd_n(const void* x, const float* gamma, const float* beta, void* y, double* stats, float eps, int act,
+               const Slab& q, hipStream_t s) {
+  if (q.vecs <= 4) return slab_fwd<T, W, 4>(x, gamma, beta, y, stats, eps, act, q, s);
+  if (q.vecs <= 8) return slab_fwd<T, W, 8>(x, gamma, beta, y, stats, eps, act, q, s);
+  return slab_fwd<T, W, 16>(x, gamma, beta, y, stats, eps, act, q, s);
+}
+size_t slab_lds(const Slab& q) {
+  const size_t row = (size_t)q.nw * q.W, segs = row > (size_t)q.threads ? row : q.threads;
+  return 8 * (q.rp * row + segs);
+}
+template <typename T, int W, int NV, int ACT>
+int slab_bwd(const void* dy, const void* x, const float* gamma, const float* beta, const double* stats, void* dx,
+             float* dgamma, float* dbeta, float* sums, const Slab& q, hipStream_t s) {
+  const size_t lds = slab_lds(q);
+  if (int rc = allow_lds<gn_slab_bwd_kernel<T, W, NV, ACT>>(lds)) return rc;
+  hipLaunchKernelGGL((gn_slab_bwd_kernel<T, W, NV, ACT>), dim3((unsigned)(q.batch * q.bundles)), dim3(q.threads), lds, s,
+                     static_cast<const T*>(dy), static_cast<const T*>(x), gamma, beta, stats, static_cast<T*>(dx), sums,
+                     q);
+  if (dgamma || dbeta)
+    hipLaunchKernelGGL(gn_param_kernel, dim3((q.C + 63) / 64), dim3(1024), 0, s, sums, q.batch, q.C, dgamma, dbeta);
+  return mmsa_launch_status();
+}
+template <typename T, int W, int ACT>
+int slab_bwd_n(const void* dy, const void* x, const float* gamma, const float* beta, const double* stats, void* dx,
+               float* dgamma, float* dbeta, float* sums, const Slab& q, hipStream_t s) {
+  if (q.vecs <= 4) return slab_bwd<T, W, 4, ACT>(dy, x, gamma, beta, stats, dx, dgamma, dbeta, sums, q, s);
+  if constexpr (W * sizeof(T) < 16)
+    return slab_bwd<T, W, 16, ACT>(dy, x, gamma, beta, stats, dx, dgamma, dbeta, sums, q, s);
+  else
+    return slab_bwd<T, W, 6, ACT>(dy, x, gamma, beta, stats, dx, dgamma, dbeta, sums, q, s);
+}
+
+// registers a thread may hold of one map: forward 64 of its 128; backward, which holds two maps and the channels'
+// coefficients, 24 in 16-byte vectors, else 16 vectors
+constexpr int FWD_REGS = 64, BWD_REGS = 24;
+
+// the three launches of a map whose groups do not fit one block
+template <typename T, bool ONCE>
+int cut_fwd(const T* x, const float* gamma, const float* beta, T* y, double* stats, double* part, long batch,
+            const Cut& cut, int dtype, float eps, int act, hipStream_t s) {
   const dim3 grid((unsigned)(batch * cut.nchunk)), block(block_of(cut));
   const size_t lds = 3 * sizeof(float) * slots_of(cut, dtype);
-  if (int rc = allow_lds(gn_stats_kernel<T>, lds)) return rc;
-  hipLaunchKernelGGL((gn_stats_kernel<T>), grid, block, lds, s, xp, cut, static_cast<double*>(scratch));
-  hipLaunchKernelGGL(gn_stats_join_kernel, dim3((unsigned)(batch * cut.G)), dim3(64), 0, s,
-                     static_cast<const double*>(scratch), cut.nchunk, cut.G, eps, stats);
+  if (int rc = allow_lds<gn_stats_kernel<T, ONCE>>(lds)) return rc;
+  hipLaunchKernelGGL((gn_stats_kernel<T, ONCE>), grid, block, lds, s, x, cut, part);
+  hipLaunchKernelGGL(gn_stats_join_kernel, dim3((unsigned)(batch * cut.G)), dim3(64), 0, s, (const double*)part,
+                     cut.nchunk, cut.G, eps, stats);
 #define GN_APPLY(A) \
-  hipLaunchKernelGGL((gn_apply_kernel<T, A>), grid, block, 0, s, xp, gamma, beta, stats, yp, cut)
+  hipLaunchKernelGGL((gn_apply_kernel<T, A, ONCE>), grid, block, 0, s, x, gamma, beta, stats, y, cut)
   switch (act) {
     case ACT_NONE: GN_APPLY(ACT_NONE); break;
     case ACT_RELU: GN_APPLY(ACT_RELU); break;
@@ -668,25 +1116,64 @@ int gn_fwd(const void* x, const float* gamma, const float* beta, void* y, double
   return mmsa_launch_status();
 }
 
-template <typename T, int ACT>
-int gn_bwd(const void* dy, const void* x, const float* gamma, const float* beta, const double* stats, void* dx,
-           float* dgamma, float* dbeta, void* scratch, long batch, const Cut& cut, int dtype, hipStream_t s) {
+template <typename T>
+int gn_fwd(const void* x, const float* gamma, const float* beta, void* y, double* stats, void* scratch, long batch,
+           const Cut& cut, int dtype, float eps, int act, hipStream_t s) {
+  Slab q;
+  if (make_slab(batch, cut.S / cut.C, cut.C, cut.G, dtype, FWD_REGS, &q)) {
+    if (q.W == Io<T>::V) return slab_fwd_n<T, Io<T>::V>(x, gamma, beta, y, stats, eps, act, q, s);
+    if constexpr (sizeof(T) == 2)
+      if (q.W == 4) return slab_fwd_n<T, 4>(x, gamma, beta, y, stats, eps, act, q, s);
+    if constexpr (sizeof(T) == 4)
+      if (q.W == 2) return slab_fwd_n<T, 2>(x, gamma, beta, y, stats, eps, act, q, s);
+    return slab_fwd_n<T, 1>(x, gamma, beta, y, stats, eps, act, q, s);
+  }
   const T* xp = static_cast<const T*>(x);
-  const T* gp = static_cast<const T*>(dy);
-  float* part = static_cast<float*>(scratch);
+  T* yp = static_cast<T*>(y);
+  double* part = static_cast<double*>(scratch);
+  if (batch * cut.S * (long)sizeof(T) > GN_CACHED)
+    return cut_fwd<T, true>(xp, gamma, beta, yp, stats, part, batch, cut, dtype, eps, act, s);
+  return cut_fwd<T, false>(xp, gamma, beta, yp, stats, part, batch, cut, dtype, eps, act, s);
+}
+
+template <typename T, int ACT, bool ONCE>
+int cut_bwd(const T* dy, const T* x, const float* gamma, const float* beta, const double* stats, T* dx, float* dgamma,
+            float* dbeta, float* part, long batch, const Cut& cut, int dtype, hipStream_t s) {
   float* sums = part + batch * cut.nchunk * cut.C * 2;
   float* coef = sums + batch * cut.C * 2;
   const dim3 grid((unsigned)(batch * cut.nchunk)), block(block_of(cut));
   const size_t lds = 2 * sizeof(float) * slots_of(cut, dtype);
-  if (int rc = allow_lds(gn_bwd_sums_kernel<T, ACT>, lds)) return rc;
-  hipLaunchKernelGGL((gn_bwd_sums_kernel<T, ACT>), grid, block, lds, s, gp, xp, gamma, beta, stats, cut, part);
+  if (int rc = allow_lds<gn_bwd_sums_kernel<T, ACT, ONCE>>(lds)) return rc;
+  hipLaunchKernelGGL((gn_bwd_sums_kernel<T, ACT, ONCE>), grid, block, lds, s, dy, x, gamma, beta, stats, cut, part);
   hipLaunchKernelGGL(gn_bwd_join_kernel, dim3((unsigned)(batch * cut.G)), dim3(256), 0, s, part, cut, gamma, sums, coef);
-  const int nparam = dgamma || dbeta ? mmsa_cdiv(cut.C, block.x) : 0;
+  const int nparam = dgamma || dbeta ? mmsa_cdiv(cut.C, 64) : 0;
   const unsigned blocks = nparam + (dx ? grid.x : 0);
   if (blocks)
-    hipLaunchKernelGGL((gn_bwd_apply_kernel<T, ACT>), dim3(blocks), block, 0, s, gp, xp, gamma, beta, stats, sums, coef,
-                       static_cast<T*>(dx), dgamma, dbeta, nparam, batch, cut);
+    hipLaunchKernelGGL((gn_bwd_apply_kernel<T, ACT, ONCE>), dim3(blocks), block, 0, s, dy, x, gamma, beta, stats, sums,
+                       coef, dx, dgamma, dbeta, nparam, batch, cut);
   return mmsa_launch_status();
+}
+
+template <typename T, int ACT>
+int gn_bwd(const void* dy, const void* x, const float* gamma, const float* beta, const double* stats, void* dx,
+           float* dgamma, float* dbeta, void* scratch, long batch, const Cut& cut, int dtype, hipStream_t s) {
+  float* part = static_cast<float*>(scratch);
+  Slab q;
+  if (make_slab(batch, cut.S / cut.C, cut.C, cut.G, dtype, BWD_REGS, &q)) {
+    if (q.W == Io<T>::V)
+      return slab_bwd_n<T, Io<T>::V, ACT>(dy, x, gamma, beta, stats, dx, dgamma, dbeta, part, q, s);
+    if constexpr (sizeof(T) == 2)
+      if (q.W == 4) return slab_bwd_n<T, 4, ACT>(dy, x, gamma, beta, stats, dx, dgamma, dbeta, part, q, s);
+    if constexpr (sizeof(T) == 4)
+      if (q.W == 2) return slab_bwd_n<T, 2, ACT>(dy, x, gamma, beta, stats, dx, dgamma, dbeta, part, q, s);
+    return slab_bwd_n<T, 1, ACT>(dy, x, gamma, beta, stats, dx, dgamma, dbeta, part, q, s);
+  }
+  const T* xp = static_cast<const T*>(x);
+  const T* gp = static_cast<const T*>(dy);
+  T* op = static_cast<T*>(dx);
+  if (2 * batch * cut.S * (long)sizeof(T) > GN_CACHED)
+    return cut_bwd<T, ACT, true>(gp, xp, gamma, beta, stats, op, dgamma, dbeta, part, batch, cut, dtype, s);
+  return cut_bwd<T, ACT, false>(gp, xp, gamma, beta, stats, op, dgamma, dbeta, part, batch, cut, dtype, s);
 }
 
 template <typename T>

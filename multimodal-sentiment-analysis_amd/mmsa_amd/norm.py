@@ -16,44 +16,43 @@ from torch.autograd.function import once_differentiable
 from . import _lib, ops
 
 
-def _rows(x: torch.Tensor) -> torch.Tensor:
-    """[B, C, *positions] -> contiguous [B, P, C]; no copy for a map in channels-last memory."""
-    B, C = x.shape[:2]
+def _channels_last(x: torch.Tensor) -> torch.Tensor:
+    """x [B, C, *positions] with its values in the order [B, *positions, C], one after another: x itself where it lies so
+    already, else a copy."""
     if x.dim() == 4:
-        return x.permute(0, 2, 3, 1).contiguous().view(B, x.shape[2] * x.shape[3], C)
-    return x.movedim(1, -1).contiguous().view(B, math.prod(x.shape[2:]), C)
-
-
-def _maps(rows: torch.Tensor, shape) -> torch.Tensor:
-    """[B, P, C] -> [B, C, *positions] in channels-last memory."""
-    if len(shape) == 4:
-        return rows.view(shape[0], shape[2], shape[3], shape[1]).permute(0, 3, 1, 2)
-    return rows.view(shape[0], *shape[2:], shape[1]).movedim(-1, 1)
+        return x if x.is_contiguous(memory_format=torch.channels_last) else x.contiguous(
+            memory_format=torch.channels_last)
+    rows = x.movedim(1, -1)
+    return x if rows.is_contiguous() else rows.contiguous().movedim(-1, 1)
 
 
 class _GroupNormActFn(torch.autograd.Function):
-    """One node from the map as the caller holds it to the result: the changes of layout are views made inside it."""
+    """One node from the map as the caller holds it to the result; x is in channels-last memory already."""
 
     @staticmethod
     def forward(ctx, x, weight, bias, groups, eps, act):
-        rows = _rows(x)
-        y = torch.empty_like(rows)
-        stats = torch.empty((rows.shape[0], groups, 2), dtype=torch.float64, device=x.device)
-        ops.group_norm_act_fwd(rows, weight, bias, y, stats, groups, eps, act)
-        ctx.save_for_backward(rows, weight, bias, stats)
-        ctx.groups, ctx.act, ctx.shape = groups, act, x.shape
-        return _maps(y, x.shape)
+        B, C = x.shape[:2]
+        y = torch.empty_like(x)
+        stats = torch.empty((B, groups, 2), dtype=torch.float64, device=x.device)
+        P = math.prod(x.shape[2:])
+        if y.numel():
+            ops._group_norm_launch_fwd(x, weight, bias, y, stats, B, P, C, groups, eps, act)
+        ctx.save_for_backward(x, weight, bias, stats)
+        ctx.args = (B, P, C, groups, act)
+        return y
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
-        rows, weight, bias, stats = ctx.saved_tensors
+        x, weight, bias, stats = ctx.saved_tensors
         want = ctx.needs_input_grad
-        dx = torch.empty_like(rows) if want[0] else None
+        if not x.numel():
+            return tuple(torch.zeros_like(t) if w else None for t, w in zip((x, weight, bias), want)) + (None,) * 3
+        dx = torch.empty_like(x) if want[0] else None
         dw = torch.empty_like(weight) if want[1] else None
         db = torch.empty_like(bias) if want[2] else None
-        ops.group_norm_act_bwd(_rows(dy), rows, weight, bias, stats, dx, dw, db, ctx.groups, ctx.act)
-        return None if dx is None else _maps(dx, ctx.shape), dw, db, None, None, None
+        ops._group_norm_launch_bwd(_channels_last(dy), x, weight, bias, stats, dx, dw, db, *ctx.args)
+        return dx, dw, db, None, None, None
 
 
 def group_norm_act(x: torch.Tensor, num_groups: int, weight=None, bias=None, eps: float = 1e-5,
@@ -69,17 +68,19 @@ def group_norm_act(x: torch.Tensor, num_groups: int, weight=None, bias=None, eps
         raise ValueError("group_norm_act: x must be [B, C, *positions]")
     if not x.is_cuda:
         raise _lib.MmsaError("group_norm_act: x must live on the GPU (the HIP kernels have no CPU path)")
+    if x.dtype not in ops.DTYPE_CODES:
+        raise TypeError(f"group_norm_act: float32, bfloat16 or float16 maps, got {x.dtype}")
     B, C = x.shape[:2]
-    if num_groups < 1 or C % num_groups or C < 1:
-        raise ValueError(f"group_norm_act: {C} channels do not divide into {num_groups} groups")
+    ops._group_norm_check(C, num_groups, activation, weight, bias)
+    x = _channels_last(x)
     if torch.is_grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad)
                                     or (bias is not None and bias.requires_grad)):
         return _GroupNormActFn.apply(x, weight, bias, num_groups, eps, activation)
-    rows = _rows(x)
-    y = torch.empty_like(rows)
-    stats = torch.empty((B, num_groups, 2), dtype=torch.float64, device=x.device)
-    ops.group_norm_act_fwd(rows, weight, bias, y, stats, num_groups, eps, activation)
-    return _maps(y, x.shape)
+    y = torch.empty_like(x)
+    if y.numel():
+        stats = torch.empty((B, num_groups, 2), dtype=torch.float64, device=x.device)
+        ops._group_norm_launch_fwd(x, weight, bias, y, stats, B, math.prod(x.shape[2:]), C, num_groups, eps, activation)
+    return y
 
 
 class GroupNormAct(nn.Module):

@@ -6,6 +6,7 @@ enqueues on torch's current HIP stream.  No wrapper computes anything itself and
 from __future__ import annotations
 
 import ctypes
+import functools
 import math
 import threading
 from typing import List, Optional, Sequence
@@ -225,26 +226,47 @@ ACTIVATIONS = {"none": 0, "relu": 1, "silu": 2, "gelu": 3}
 DTYPE_CODES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 
 
-def _group_norm_args(x, gamma, beta, groups, act):
-    if x.dim() != 3:
-        raise ValueError("group_norm_act: x must be [B, positions, channels]")
-    if x.dtype not in DTYPE_CODES:
-        raise TypeError(f"group_norm_act: float32, bfloat16 or float16 maps, got {x.dtype}")
+def _group_norm_check(C, groups, act, gamma, beta):
     if act not in ACTIVATIONS:
         raise ValueError(f"group_norm_act: activation {act!r} is none of {', '.join(ACTIVATIONS)}")
-    B, P, C = x.shape
     if groups < 1 or C < 1 or C % groups:
         raise ValueError(f"group_norm_act: {C} channels do not divide into {groups} groups")
     for t, name in ((gamma, "weight"), (beta, "bias")):
         if t is not None and tuple(t.shape) != (C,):
             raise ValueError(f"group_norm_act: {name} must be [{C}]")
-    return B, P, C
 
 
-def _group_norm_scratch(x, groups):
-    B, P, C = x.shape
-    n = _lib.query("mmsa_group_norm_act_scratch_bytes", B, P, C, groups, DTYPE_CODES[x.dtype])
-    return torch.empty(((n + 7) // 8,), dtype=torch.float64, device=x.device)
+def _group_norm_args(x, gamma, beta, groups, act):
+    if x.dim() != 3:
+        raise ValueError("group_norm_act: x must be [B, positions, channels]")
+    if x.dtype not in DTYPE_CODES:
+        raise TypeError(f"group_norm_act: float32, bfloat16 or float16 maps, got {x.dtype}")
+    _group_norm_check(x.shape[2], groups, act, gamma, beta)
+    return x.shape
+
+
+@functools.lru_cache(maxsize=256)
+def _group_norm_scratch_doubles(B, P, C, groups, code):
+    return (_lib.query("mmsa_group_norm_act_scratch_bytes", B, P, C, groups, code) + 7) // 8
+
+
+def _group_norm_launch_fwd(x, gamma, beta, y, stats, B, P, C, groups, eps, act):
+    """The launch alone, for a caller that has checked layouts itself: x and y hold [B, P, C] one value after another."""
+    code = DTYPE_CODES[x.dtype]
+    scratch = torch.empty(_group_norm_scratch_doubles(B, P, C, groups, code), dtype=torch.float64, device=x.device)
+    _OPERANDS.dev = x.get_device()
+    _lib.call("mmsa_group_norm_act_fwd", x.data_ptr(), _opt(gamma, F32, "weight"), _opt(beta, F32, "bias"), y.data_ptr(),
+              stats.data_ptr(), scratch.data_ptr(), B, P, C, groups, eps, ACTIVATIONS[act], code, _stream())
+
+
+def _group_norm_launch_bwd(dy, x, gamma, beta, stats, dx, dgamma, dbeta, B, P, C, groups, act):
+    code = DTYPE_CODES[x.dtype]
+    scratch = torch.empty(_group_norm_scratch_doubles(B, P, C, groups, code), dtype=torch.float64, device=x.device)
+    _OPERANDS.dev = x.get_device()
+    _lib.call("mmsa_group_norm_act_bwd", dy.data_ptr(), x.data_ptr(), None if gamma is None else gamma.data_ptr(),
+              None if beta is None else beta.data_ptr(), stats.data_ptr(), None if dx is None else dx.data_ptr(),
+              None if dgamma is None else dgamma.data_ptr(), None if dbeta is None else dbeta.data_ptr(),
+              scratch.data_ptr(), B, P, C, groups, ACTIVATIONS[act], code, _stream())
 
 
 def group_norm_act_fwd(x, gamma, beta, y, stats, groups: int, eps: float = 1e-5, act: str = "none"):
@@ -255,9 +277,8 @@ def group_norm_act_fwd(x, gamma, beta, y, stats, groups: int, eps: float = 1e-5,
         raise ValueError("group_norm_act_fwd: y like x, stats [B, groups, 2]")
     if x.numel() == 0:
         return y
-    _lib.call("mmsa_group_norm_act_fwd", _chk(x, x.dtype, "x"), _opt(gamma, F32, "weight"), _opt(beta, F32, "bias"),
-              _chk(y, x.dtype, "y"), _chk(stats, torch.float64, "stats"), _group_norm_scratch(x, groups).data_ptr(),
-              B, P, C, groups, eps, ACTIVATIONS[act], DTYPE_CODES[x.dtype], _stream())
+    _chk(y, x.dtype, "y"), _chk(stats, torch.float64, "stats"), _chk(x, x.dtype, "x")
+    _group_norm_launch_fwd(x, gamma, beta, y, stats, B, P, C, groups, eps, act)
     return y
 
 
@@ -274,10 +295,11 @@ def group_norm_act_bwd(dy, x, gamma, beta, stats, dx, dgamma, dbeta, groups: int
             if t is not None:
                 t.zero_()
         return
-    _lib.call("mmsa_group_norm_act_bwd", _chk(dy, x.dtype, "dy"), _chk(x, x.dtype, "x"), _opt(gamma, F32, "weight"),
-              _opt(beta, F32, "bias"), _chk(stats, torch.float64, "stats"), _opt(dx, x.dtype, "dx"),
-              _opt(dgamma, F32, "dgamma"), _opt(dbeta, F32, "dbeta"), _group_norm_scratch(x, groups).data_ptr(),
-              B, P, C, groups, ACTIVATIONS[act], DTYPE_CODES[x.dtype], _stream())
+    for t, dtype, name in ((dy, x.dtype, "dy"), (gamma, F32, "weight"), (beta, F32, "bias"),
+                           (stats, torch.float64, "stats"), (dx, x.dtype, "dx"), (dgamma, F32, "dgamma"),
+                           (dbeta, F32, "dbeta"), (x, x.dtype, "x")):
+        _opt(t, dtype, name)
+    _group_norm_launch_bwd(dy, x, gamma, beta, stats, dx, dgamma, dbeta, B, P, C, groups, act)
 
 
 # ---------------------------------------------------------------------------------------------- convolution
