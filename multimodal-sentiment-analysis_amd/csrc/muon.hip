@@ -327,6 +327,7 @@ struct Tile {
   static constexpr int OPER = BT * ROW;
   static constexpr int RING = 4;                        // LDS buffers
   static constexpr int LOADS = BT * G / 32;             // a thread's loads per step
+  static constexpr int SUMS = BT == 256 ? 1 : 2;        // accumulators per value
   static constexpr int PASSES = BT == 256 ? 2 : 1;      // rounds in which the results leave through LDS
   static constexpr int OUTROW = BT * 4 + 16;            // an output row of pairs in LDS, padded against bank conflicts
   static constexpr int LDS = RING * 2 * OPER > BT / PASSES * OUTROW ? RING * 2 * OPER : BT / PASSES * OUTROW;
@@ -353,10 +354,23 @@ struct Fragments {
   f16x8 qh[Tile<BT>::G][Tile<BT>::W], ql[Tile<BT>::G][Tile<BT>::W];
 };
 
+//
+// A matrix instruction rounds twice into its fp32 accumulator.  The products hi lo + lo hi are 2^-11 of hi hi: in an
+// accumulator of their own they round at that scale, and the main one is rounded a third as often (0.6 of the error at
+// K = 2048).  The 256 x 256 tile has no registers left for that.
 template <int BT>
 __device__ __forceinline__ void multiply(f32x16 (&acc)[Tile<BT>::W][Tile<BT>::W], char* lds, const char* P,
                                          const char* Q, long pitch, int nk32) {
   typedef Tile<BT> S;
+  f32x16 low[S::SUMS == 2 ? S::W : 1][S::SUMS == 2 ? S::W : 1];
+  if (S::SUMS == 2) {
+#pragma unroll
+    for (int x = 0; x < (S::SUMS == 2 ? S::W : 1); ++x)
+#pragma unroll
+      for (int y = 0; y < (S::SUMS == 2 ? S::W : 1); ++y)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) low[x][y][e] = 0.f;
+  }
   constexpr int W = S::W, G = S::G, ROW = S::ROW, OPER = S::OPER, LOADS = S::LOADS;
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
   const int nk = nk32 * 2 / G;
@@ -395,15 +409,28 @@ __device__ __forceinline__ void multiply(f32x16 (&acc)[Tile<BT>::W][Tile<BT>::W]
 #pragma unroll
       for (int x = 0; x < W; ++x) {
 #pragma unroll
-        for (int y = 0; y < W; ++y)
-          acc[x][y] = __builtin_amdgcn_mfma_f32_32x32x16_f16(f.pl[s][x], f.qh[s][y], acc[x][y], 0, 0, 0);
+        for (int y = 0; y < W; ++y) {
+          f32x16& to = S::SUMS == 2 ? low[S::SUMS == 2 ? x : 0][S::SUMS == 2 ? y : 0] : acc[x][y];
+          to = __builtin_amdgcn_mfma_f32_32x32x16_f16(f.pl[s][x], f.qh[s][y], to, 0, 0, 0);
+        }
 #pragma unroll
-        for (int y = 0; y < W; ++y)
-          acc[x][y] = __builtin_amdgcn_mfma_f32_32x32x16_f16(f.ph[s][x], f.ql[s][y], acc[x][y], 0, 0, 0);
+        for (int y = 0; y < W; ++y) {
+          f32x16& to = S::SUMS == 2 ? low[S::SUMS == 2 ? x : 0][S::SUMS == 2 ? y : 0] : acc[x][y];
+          to = __builtin_amdgcn_mfma_f32_32x32x16_f16(f.ph[s][x], f.ql[s][y], to, 0, 0, 0);
+        }
 #pragma unroll
         for (int y = 0; y < W; ++y)
           acc[x][y] = __builtin_amdgcn_mfma_f32_32x32x16_f16(f.ph[s][x], f.qh[s][y], acc[x][y], 0, 0, 0);
       }
+  };
+  auto join = [&]() {
+    if (S::SUMS == 1) return;
+#pragma unroll
+    for (int x = 0; x < (S::SUMS == 2 ? W : 0); ++x)
+#pragma unroll
+      for (int y = 0; y < (S::SUMS == 2 ? W : 0); ++y)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) acc[x][y][e] += low[x][y][e];
   };
   // Step k: step k + 1 has arrived for all waves, so its fragments can be read; the buffer of step k + 3 held step
   // k - 1, whose fragments every wave had before it came here.  The reads and loads are spread over the matrix
@@ -435,6 +462,7 @@ __device__ __forceinline__ void multiply(f32x16 (&acc)[Tile<BT>::W][Tile<BT>::W]
     fetch(b, 1);
     compute(a);
     compute(b);
+    join();
     return;
   }
   stage(2);
@@ -454,6 +482,7 @@ __device__ __forceinline__ void multiply(f32x16 (&acc)[Tile<BT>::W][Tile<BT>::W]
   compute(a);
   __builtin_amdgcn_sched_barrier(0);
   compute(b);
+  join();
 }
 
 // D = P Q^T for one BT x BT tile of one matrix.
@@ -505,7 +534,7 @@ __global__ __launch_bounds__(256, BT == 256 || Tile<BT>::LDS > 81920 ? 1 : 2) vo
   multiply<BT>(acc, lds, P + (long)ti * BT * pitch + k_lo * 128l, Q + (long)tj * BT * pitch + k_lo * 128l, pitch, nk);
   const int wi = w >> 1, wj = w & 1, fr = lane & 31, half = lane >> 5;
   // register e of a wave's tile (x, y): row (e & 3) + 8 (e >> 2) + 4 half, column fr
-  if (MODE <= TO_B && BT < 256 && nsplit > 1) {
+  if (MODE <= TO_B && nsplit > 1) {
     float* o = ws_part(q) + ((long)tile * nsplit + part) * (BT * BT) + tid;
 #pragma unroll
     for (int x = 0; x < W; ++x)
@@ -805,14 +834,14 @@ void make_plan(const int* rows, const int* cols, Group* gr, Plan* pl) {
     long share = 0;
     pl->bt[ph] = 0;
     for (const TileCost& c : COST) {
-      if (c.bt > pad) break;
+      if (c.bt > pad || c.bt == 256) break;       // errors of T count most: tiles with two accumulators only
       long work = 0, most = 0;
       for (int i = 0; i < n; ++i) {
         const long k = (ph == TO_T ? gr->mat[i].np : gr->mat[i].mp) / 32;
         work += tri(gr->mat[i].mp / c.bt) * k;
         if (k > most) most = k;
       }
-      for (int rounds = 0; rounds <= (c.bt == 256 ? 0 : 4); ++rounds) {       // 0: whole
+      for (int rounds = 0; rounds <= 4; ++rounds) {       // 0: whole
         long kper = most;
         if (rounds) {
           kper = (work / (rounds * c.slots) + 2) & ~1l;
@@ -878,9 +907,13 @@ template <typename T, int MODE>
 void launch_product(const Plan& pl, const Group* dev, int step, const Step& st, hipStream_t s) {
   constexpr int PHASE = MODE < TO_X ? MODE : TO_X;
   const dim3 grid(pl.blocks[PH_PRODUCT + PHASE]);
-  if (pl.bt[PHASE] == 256)
-    hipLaunchKernelGGL((product_kernel<T, 256, MODE>), grid, dim3(256), 0, s, dev, step, step & 1, st.decay, st.rate);
-  else if (pl.bt[PHASE] == 128)
+  if constexpr (MODE >= TO_X) {
+    if (pl.bt[PHASE] == 256) {
+      hipLaunchKernelGGL((product_kernel<T, 256, MODE>), grid, dim3(256), 0, s, dev, step, step & 1, st.decay, st.rate);
+      return;
+    }
+  }
+  if (pl.bt[PHASE] == 128)
     hipLaunchKernelGGL((product_kernel<T, 128, MODE>), grid, dim3(256), 0, s, dev, step, step & 1, st.decay, st.rate);
   else
     hipLaunchKernelGGL((product_kernel<T, 64, MODE>), grid, dim3(256), 0, s, dev, step, step & 1, st.decay, st.rate);
