@@ -731,6 +731,261 @@ __global__ __launch_bounds__(256) void join_kernel(const Group* __restrict__ grp
   *reinterpret_cast<f16x4*>(o + 32) = lo;
 }
 
+// ---- matrices that fit one block
+// m <= 64 and n <= 32 * 8 * NT: the whole iteration in one launch, a block of eight waves per matrix.  At these sizes the
+// seventeen dependent launches of the general path are all there is to its time (64 x 288: 72 us).
+// X lives in registers: wave w holds the column tiles w, w + 8, ... of 32 columns as the pairs that the product B X
+// takes and gives back -- the accumulator of a product (lane: column; registers: rows 4 h + (e & 3) + 8 (e >> 2) of
+// each 32) is the right operand of the next one with its K index in that order, and the left operand, B, is read from
+// LDS in the same order.  X X^T needs X by rows: a wave turns its tiles over in LDS, and the waves' parts are added up
+// there.  In LDS a pair is one 32-bit word, lo << 16 | hi.
+constexpr int SMALL_M = 64, SMALL_NT = 3, SMALL_N = 256 * SMALL_NT;
+constexpr int TURN_ROW = 36, SQUARE_ROW = 68;          // words of a row, padded against bank conflicts
+constexpr int WAVE_WORDS = 3 * 16 * 64;                // a wave's part of X X^T: three of the four 32 x 32 tiles
+static_assert(64 * TURN_ROW <= WAVE_WORDS, "a wave's turning buffer and its part of the sum share their place");
+
+__device__ __forceinline__ unsigned to_pair(float v) {
+  const _Float16 p[2] = {(_Float16)v, (_Float16)(v - (float)(_Float16)v)};
+  unsigned u;
+  __builtin_memcpy(&u, p, 4);
+  return u;
+}
+// eight pairs -> the two fragments
+__device__ __forceinline__ void from_pairs(const uint4& a, const uint4& b, f16x8& hi, f16x8& lo) {
+  const unsigned w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+  unsigned h[4], l[4];
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    h[k] = __builtin_amdgcn_perm(w[2 * k + 1], w[2 * k], 0x05040100);
+    l[k] = __builtin_amdgcn_perm(w[2 * k + 1], w[2 * k], 0x07060302);
+  }
+  __builtin_memcpy(&hi, h, 16);
+  __builtin_memcpy(&lo, l, 16);
+}
+// one product of pairs, the low ones in an accumulator of their own
+__device__ __forceinline__ void pair_product(const f16x8& ph, const f16x8& pl, const f16x8& qh, const f16x8& ql,
+                                             f32x16& acc, f32x16& low) {
+  low = __builtin_amdgcn_mfma_f32_32x32x16_f16(pl, qh, low, 0, 0, 0);
+  acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(ph, qh, acc, 0, 0, 0);
+  low = __builtin_amdgcn_mfma_f32_32x32x16_f16(ph, ql, low, 0, 0, 0);
+}
+
+// a value the compiler cannot see through: without it the double -> float -> half roundings of the first pairs become one
+// long emulated conversion each, and the addresses of the loads are kept, spilled, for the stores at the end
+template <typename V>
+__device__ __forceinline__ V opaque(V v) {
+  asm volatile("" : "+v"(v));
+  return v;
+}
+
+template <typename T, bool MOM, int NT>
+__global__ __launch_bounds__(512) void small_kernel(const Group gr, float mu, float one_minus_mu, int nesterov,
+                                                    float eps, int steps, float decay, float rate) {
+  extern __shared__ unsigned words[];
+  __shared__ double red[16];
+  const Mat q = gr.mat[blockIdx.x];
+  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, col = lane & 31, half = lane >> 5;
+  unsigned* own = words + w * WAVE_WORDS;
+  unsigned* sq_t = words + 8 * WAVE_WORDS;
+  unsigned* sq_b = sq_t + 64 * SQUARE_ROW;
+  const bool tall = q.rows > q.cols;
+  // element e of row tile x of column tile t: row i, column j, and its place in the caller's matrix (0 behind the edges,
+  // so that every load can be issued without a branch: a branch would wait for each in turn)
+  auto row_of = [&](int x, int e) { return x * 32 + (e & 3) + 8 * (e >> 2) + 4 * half; };
+  auto col_of = [&](int t) { return (t * 8 + w) * 32 + col; };
+  const unsigned si = tall ? 1 : q.cols, sj = tall ? q.cols : 1;
+  unsigned corner = 4 * half * si + (w * 32 + col) * sj;
+  int below = q.m - 4 * half, right = q.n - w * 32 - col;      // rows and columns there are from the corner on
+  auto inside = [&](int x, int e, int t) { return x * 32 + (e & 3) + 8 * (e >> 2) < below && t * 256 < right; };
+  auto place = [&](int x, int e, int t) {
+    const unsigned at = corner + (x * 32 + (e & 3) + 8 * (e >> 2)) * si + t * 256 * sj;
+    return inside(x, e, t) ? at : 0u;
+  };
+  float u[NT][2][16];
+#pragma unroll
+  for (int t = 0; t < NT; ++t)
+#pragma unroll
+    for (int x = 0; x < 2; ++x)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) u[t][x][e] = El<T>::get(q.g, place(x, e, t));
+  if (MOM) {
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        float m[16];
+#pragma unroll
+        for (int e = 0; e < 16; ++e) m[e] = q.mom[place(x, e, t)];
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          const float g = u[t][x][e];
+          m[e] = fmaf(one_minus_mu, g - m[e], m[e]);
+          if (inside(x, e, t)) q.mom[place(x, e, t)] = m[e];
+          u[t][x][e] = direction(g, m[e], mu, nesterov);
+        }
+      }
+  }
+  double ss = 0.0;
+#pragma unroll
+  for (int t = 0; t < NT; ++t)
+#pragma unroll
+    for (int x = 0; x < 2; ++x)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        if (!inside(x, e, t)) u[t][x][e] = 0.f;
+        ss += (double)u[t][x][e] * (double)u[t][x][e];
+      }
+  ss = block_sum_d(ss, red);
+  const double norm = sqrt(ss);
+  const double size = norm > (double)eps ? norm : (norm != norm ? norm : (double)eps);
+  double r = norm / size;
+  int k0 = extra_scale(r);
+  const double mul0 = ldexp(1.0 / size, NS_SCALE + k0);
+  f16x8 xh[NT][4], xl[NT][4];
+  auto keep = [&](int t, int x, int e, float v) {
+    const _Float16 hi = (_Float16)v;
+    xh[t][x * 2 + (e >> 3)][e & 7] = hi;
+    xl[t][x * 2 + (e >> 3)][e & 7] = (_Float16)(v - (float)hi);
+  };
+#pragma unroll
+  for (int t = 0; t < NT; ++t)
+#pragma unroll
+    for (int x = 0; x < 2; ++x)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) keep(t, x, e, opaque((float)((double)u[t][x][e] * mul0)));
+
+  for (int step = 0; step < steps; ++step) {
+    r = fmin((double)NS_A * r, 1.2025);
+    const int k1 = extra_scale(r);
+    // T = X X^T + shift: tiles (0, 0), (1, 0), (1, 1)
+    f32x16 acc[3], low[3];
+#pragma unroll
+    for (int k = 0; k < 3; ++k)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) acc[k][e] = low[k][e] = 0.f;
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      if ((t * 8 + w) * 32 >= q.n) break;                    // uniform in the wave: the tile holds padding only
+#pragma unroll
+      for (int x = 0; x < 2; ++x)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          const _Float16 p[2] = {xh[t][x * 2 + (e >> 3)][e & 7], xl[t][x * 2 + (e >> 3)][e & 7]};
+          unsigned v;
+          __builtin_memcpy(&v, p, 4);
+          own[row_of(x, e) * TURN_ROW + col] = v;
+        }
+      __builtin_amdgcn_wave_barrier();
+#pragma unroll
+      for (int g = 0; g < 2; ++g) {
+        f16x8 ph[2], pl[2];
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+          const uint4* p = reinterpret_cast<const uint4*>(own + (x * 32 + col) * TURN_ROW + g * 16 + half * 8);
+          from_pairs(p[0], p[1], ph[x], pl[x]);
+        }
+        pair_product(ph[0], pl[0], ph[0], pl[0], acc[0], low[0]);
+        pair_product(ph[1], pl[1], ph[0], pl[0], acc[1], low[1]);
+        pair_product(ph[1], pl[1], ph[1], pl[1], acc[2], low[2]);
+      }
+      __builtin_amdgcn_wave_barrier();
+    }
+#pragma unroll
+    for (int k = 0; k < 3; ++k)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) own[(k * 16 + e) * 64 + lane] = __float_as_uint(acc[k][e] + low[k][e]);
+    __syncthreads();
+    const float smul = ldexpf(1.f, -NS_SCALE - 2 * k0);
+#pragma unroll
+    for (int n = 0; n < WAVE_WORDS / 512; ++n) {
+      const int at = n * 512 + tid, k = at >> 10, e = (at >> 6) & 15;
+      float v = 0.f;
+#pragma unroll
+      for (int o = 0; o < 8; ++o) v += __uint_as_float(words[o * WAVE_WORDS + at]);
+      const int i = row_of(k ? 1 : 0, e), j = (k == 2 ? 32 : 0) + col;
+      v *= smul;
+      if (i == j) v += ldexpf(NS_SHIFT, NS_SCALE);
+      const unsigned p = to_pair(v);
+      sq_t[i * SQUARE_ROW + j] = p;
+      if (k == 1) sq_t[j * SQUARE_ROW + i] = p;
+    }
+    __syncthreads();
+    // B = c T T + rest: one 32 x 32 tile for each of four waves
+    if (w < 4) {
+      const int x = w >> 1, y = w & 1;
+      f32x16 b, bl;
+#pragma unroll
+      for (int e = 0; e < 16; ++e) b[e] = bl[e] = 0.f;
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        f16x8 ph, pl, qh, ql;
+        const uint4* p = reinterpret_cast<const uint4*>(sq_t + (x * 32 + col) * SQUARE_ROW + g * 16 + half * 8);
+        const uint4* t = reinterpret_cast<const uint4*>(sq_t + (y * 32 + col) * SQUARE_ROW + g * 16 + half * 8);
+        from_pairs(p[0], p[1], ph, pl);
+        from_pairs(t[0], t[1], qh, ql);
+        pair_product(ph, pl, qh, ql, b, bl);
+      }
+      const float bmul = ldexpf(NS_C, -NS_SCALE);
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        const int i = row_of(x, e), j = y * 32 + col;
+        sq_b[i * SQUARE_ROW + j] = to_pair((b[e] + bl[e]) * bmul + (i == j ? ldexpf(NS_REST, NS_SCALE) : 0.f));
+      }
+    }
+    __syncthreads();
+    // X = B X
+    const float xmul = ldexpf(1.f, k1 - k0 - NS_SCALE);
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      if ((t * 8 + w) * 32 >= q.n) break;
+      f32x16 d[2], dl[2];
+#pragma unroll
+      for (int x = 0; x < 2; ++x)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) d[x][e] = dl[x][e] = 0.f;
+#pragma unroll
+      for (int g = 0; g < 4; ++g)
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+          f16x8 ph, pl;
+          const uint4* p = reinterpret_cast<const uint4*>(sq_b + (x * 32 + col) * SQUARE_ROW + g * 16 + half * 4);
+          from_pairs(p[0], p[2], ph, pl);                    // rows 4 h + 0..3 and 8 + 4 h + 0..3 of these sixteen
+          pair_product(ph, pl, xh[t][g], xl[t][g], d[x], dl[x]);
+        }
+#pragma unroll
+      for (int x = 0; x < 2; ++x)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) keep(t, x, e, (d[x][e] + dl[x][e]) * xmul);
+    }
+    k0 = k1;
+  }
+  const float omul = ldexpf(1.f, -NS_SCALE - k0);
+  corner = opaque(corner);
+  below = opaque(below);
+  right = opaque(right);
+#pragma unroll
+  for (int t = 0; t < NT; ++t)
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+      float* p = static_cast<float*>(q.out);
+      float old[16];
+      if (MOM) {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) old[e] = p[place(x, e, t)];
+      }
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        const int g = x * 2 + (e >> 3);
+        const float v = ((float)xh[t][g][e & 7] + (float)xl[t][g][e & 7]) * omul;
+        if (!inside(x, e, t)) continue;
+        if (MOM)
+          p[place(x, e, t)] = fmaf(old[e], decay, -rate * q.adjust * v);
+        else
+          El<T>::put(q.out, place(x, e, t), v);
+      }
+    }
+}
+
 // ---- host side
 constexpr int MAX_SIDE = 1 << 20;
 constexpr long MAX_VALUES = 1l << 31;
@@ -928,6 +1183,38 @@ void launch_join(const Plan& pl, const Group* dev, int step, hipStream_t s) {
     hipLaunchKernelGGL((join_kernel<64, MODE>), dim3(blocks), dim3(256), 0, s, dev, step);
 }
 
+// raising a kernel's LDS limit belongs to the device that is current
+template <auto kernel>
+int allow_lds(size_t bytes) {
+  static PerDeviceOnce once;
+  if (once.pending()) {
+    if (hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize,
+                            (int)bytes) != hipSuccess)
+      return MMSA_ERR_LAUNCH;
+    once.done();
+  }
+  return MMSA_OK;
+}
+
+bool all_small(const int* rows, const int* cols, int count, int* longest) {
+  *longest = 0;
+  for (int i = 0; i < count; ++i) {
+    const int m = rows[i] < cols[i] ? rows[i] : cols[i], n = rows[i] < cols[i] ? cols[i] : rows[i];
+    if (m > SMALL_M || n > SMALL_N) return false;
+    if (n > *longest) *longest = n;
+  }
+  return true;
+}
+
+template <typename T, bool MOM, int NT>
+int launch_small(const Group& gr, const Step& st, hipStream_t s) {
+  constexpr size_t lds = 4 * (8 * WAVE_WORDS + 2 * 64 * SQUARE_ROW);
+  if (int rc = allow_lds<small_kernel<T, MOM, NT>>(lds)) return rc;
+  hipLaunchKernelGGL((small_kernel<T, MOM, NT>), dim3(gr.count), dim3(512), lds, s, gr, st.mu, st.one_minus_mu,
+                     st.nesterov, st.eps, st.steps, st.decay, st.rate);
+  return mmsa_launch_status();
+}
+
 template <typename T, bool MOM>
 int run_all(const void* const* src, void* const* dst, void* const* mom, const int* rows, const int* cols, int count,
             const Step& st, void* scratch, hipStream_t s) {
@@ -937,6 +1224,8 @@ int run_all(const void* const* src, void* const* dst, void* const* mom, const in
     gr.count = count - i0 < GROUP ? count - i0 : GROUP;
     Plan pl;
     make_plan(rows + i0, cols + i0, &gr, &pl);
+    int longest;
+    const bool small = all_small(rows + i0, cols + i0, gr.count, &longest);
     for (int i = 0; i < gr.count; ++i) {
       Mat& q = gr.mat[i];
       const int at = i0 + pl.from[i];
@@ -945,6 +1234,13 @@ int run_all(const void* const* src, void* const* dst, void* const* mom, const in
       q.mom = mom ? static_cast<float*>(mom[at]) : nullptr;
       q.ws = static_cast<char*>(scratch) + q.ws_off;
       q.adjust = q.rows > q.cols ? sqrtf((float)q.rows / (float)q.cols) : 1.f;
+    }
+    if (small) {
+      const int rc = longest <= 256   ? launch_small<T, MOM, 1>(gr, st, s)
+                     : longest <= 512 ? launch_small<T, MOM, 2>(gr, st, s)
+                                      : launch_small<T, MOM, SMALL_NT>(gr, st, s);
+      if (rc) return rc;
+      continue;
     }
     Group* dev = static_cast<Group*>(scratch);
     double* parts = reinterpret_cast<double*>(static_cast<char*>(scratch) + (sizeof(Group) + 127) / 128 * 128);

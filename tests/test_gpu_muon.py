@@ -64,6 +64,32 @@ def test_orthogonalize_matches_the_formula(shape, dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("longest", [256, 257, 512, 513, 768, 769])
+def test_lists_of_small_matrices(longest):
+    """Up to 64 rows and 768 columns (or the transpose) a matrix is one block's work, if all of its list are; one longer
+    matrix sends the list the general way."""
+    from mmsa_amd.muon import muon_step, orthogonalize
+    shapes = [(64, longest), (longest, 3), (1, 1), (33, 32), (50, 64), (64, 64), (17, 255)] + [(5 + i, 40) for i in range(30)]
+    gs = [grad(*s, seed=i) for i, s in enumerate(shapes)]
+    gs[3][7, 7] = float("nan")
+    gs[4].zero_()
+    for s, g, o in zip(shapes, gs, orthogonalize(gs)):
+        if s == (33, 32):
+            assert bool(o.isnan().all())
+        elif s == (50, 64):
+            assert float(o.abs().max()) == 0.0
+        else:
+            close(o, ns64(g), tol(s))
+    for g, tiny in ((gs[0], 1e-9), (gs[1], 1e-12)):
+        close(orthogonalize(g * tiny), ns64(g * tiny), tol(shapes[0]))
+    p, m = gs[0].clone(), gs[0] * 0.5
+    want, mom, o = muon64(p, gs[0], m, 0.02, 0.1, 0.9, True)
+    muon_step([p], [gs[0]], [m], lr=0.02, weight_decay=0.1, momentum=0.9)
+    assert float((p.double() - want).norm()) <= 0.02 * (tol(shapes[0]) + 248 * U) * float(o.norm()) + 4 * U * float(want.norm())
+    assert float((m.double() - mom).abs().max()) <= 4 * U * float(gs[0].abs().max())
+
+
+@pytest.mark.gpu
 def test_a_large_matrix():
     from mmsa_amd.muon import orthogonalize
     for shape in ((2048, 2100), (4097, 700)):
