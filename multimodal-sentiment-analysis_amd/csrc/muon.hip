@@ -58,7 +58,8 @@ struct Mat {
 struct Group {
   Mat mat[GROUP];
   int first[PH_COUNT][GROUP];   // first block of every matrix in each kind of launch
-  int count, pad_;
+  int count;
+  int even[3];                  // all blocks of the T, B, X product have the same K
 };
 static_assert(sizeof(Group) < 4096 - 256, "kernel arguments are limited to 4 KiB");
 
@@ -311,8 +312,9 @@ __device__ __forceinline__ float diagonal() {
   return ldexpf(MODE == TO_T ? NS_SHIFT : NS_REST, NS_SCALE);
 }
 
-// The order in which a matrix's tiles are given to its blocks: consecutive blocks go to the eight XCDs in turn, each
-// with an L2 of its own, so every XCD gets one consecutive run of tiles (whose operand rows it shares).
+// The order in which tiles are given to blocks: consecutive blocks go to the eight XCDs in turn, each with an L2 of its
+// own, so every XCD gets one consecutive run of tiles (whose operand rows it shares) -- of all the launch's tiles where
+// they take equally long, else of every matrix's, so that no XCD gets the long ones.
 __device__ __forceinline__ int xcd_order(int l, int n) {
   const int per = n >> 3;
   return l < per << 3 ? (l & 7) * per + (l >> 3) : l;
@@ -497,16 +499,18 @@ __global__ __launch_bounds__(256, BT == 256 || Tile<BT>::LDS > 81920 ? 1 : 2) vo
   __shared__ __attribute__((aligned(128))) char lds[S::LDS];
   const Group& gr = *grp;
   constexpr int PHASE = MODE < TO_X ? MODE : TO_X;
-  const int mi = find_mat(gr.first[PH_PRODUCT + PHASE], gr.count, blockIdx.x);
+  const bool even = gr.even[PHASE];
+  const int block = even ? xcd_order(blockIdx.x, gridDim.x) : blockIdx.x;
+  const int mi = find_mat(gr.first[PH_PRODUCT + PHASE], gr.count, block);
   const Mat& q = gr.mat[mi];
-  const int b = blockIdx.x - gr.first[PH_PRODUCT + PHASE][mi];
+  const int b = block - gr.first[PH_PRODUCT + PHASE][mi];
   const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
   const int K = MODE == TO_T ? q.np : q.mp;
   int ti, tj, k_lo = 0, nk = K / 32, part = 0, nsplit = 1, tile = 0;
   if (MODE <= TO_B) {
     const int nt = q.mp / BT;
     nsplit = q.nsplit[PHASE];
-    const int l = xcd_order(b, nt * (nt + 1) / 2 * nsplit);
+    const int l = even ? b : xcd_order(b, nt * (nt + 1) / 2 * nsplit);
     tile = l / nsplit;
     part = l % nsplit;
     lower_tile(tile, ti, tj);
@@ -516,7 +520,7 @@ __global__ __launch_bounds__(256, BT == 256 || Tile<BT>::LDS > 81920 ? 1 : 2) vo
   } else {
     // bands of eight tile rows, column by column
     const int mt = q.mp / BT, nt = q.np / BT;
-    const int l = xcd_order(b, mt * nt);
+    const int l = even ? b : xcd_order(b, mt * nt);
     const int band = l / (8 * nt), rows = mt - band * 8 < 8 ? mt - band * 8 : 8, r = l - band * 8 * nt;
     ti = band * 8 + r % rows;
     tj = r / rows;
@@ -1146,6 +1150,13 @@ void make_plan(const int* rows, const int* cols, Group* gr, Plan* pl) {
     }
     total[PH_PRODUCT + TO_X] += (q.mp / pad) * (q.np / pad);
     bytes += mat_bytes(q) + 4 * part_floats;
+  }
+  for (int ph = 0; ph < 3; ++ph) {
+    gr->even[ph] = 1;
+    for (int i = 1; i < n; ++i) {
+      const Mat &q = gr->mat[i], &o = gr->mat[0];
+      if ((ph == TO_T ? q.np != o.np : q.mp != o.mp) || (ph < TO_X && q.nsplit[ph] != o.nsplit[ph])) gr->even[ph] = 0;
+    }
   }
   for (int p = 0; p < PH_COUNT; ++p) pl->blocks[p] = total[p];
   pl->bytes = bytes;
