@@ -8,7 +8,7 @@
  *
  * Conventions
  *   - every pointer is DEVICE memory unless the name ends in _host or the comment says "host";
- *   - fp32 everywhere, token ids / labels / num_batches_tracked are int64 (long long);
+ *   - fp32 (the group normalisation and the orthogonalisation take bf16 and fp16 too), token ids / labels / num_batches_tracked are int64 (long long);
  *   - activations are channels-last [B][H][W][C]; weights arrive in the reference's layouts;
  *   - `stream` is a hipStream_t (0 = default stream); kernels are only enqueued, never synchronised;
  *   - return value: 0 on success, MMSA_ERR_ARG (-1) for rejected arguments (nothing was launched),
@@ -459,8 +459,8 @@ MMSA_API int mmsa_group_norm_act_bwd(const void* dy, const void* x, const float*
 /* ---- orthogonalised updates (beside mmsa_adamw_step: the update of the weight matrices) ----------------------------
  * dst = X_steps of  X_0 = src / max(||src||_F, eps),  X <- (a I + b S + c S S) X,  S = X X^T  (on src^T where src has
  * more rows than columns), (a, b, c) = (3.4445, -4.775, 2.0315): singular values are driven towards 1.  `count`
- * matrices of one dtype (MMSA_F32 / MMSA_BF16 / MMSA_F16), row-major contiguous [rows][cols], in shared launches; src
- * and dst may be the same.  *_host: host arrays of `count` device pointers / sizes.  1 <= steps <= 16.  A zero matrix
+ * matrices of one dtype (MMSA_F32 / MMSA_BF16 / MMSA_F16), row-major contiguous [rows][cols], in shared launches;
+ * dst[i] may be src[i], apart from that no destination shares memory with another operand.  *_host: host arrays of `count` device pointers / sizes.  1 <= steps <= 16.  A zero matrix
  * gives zeros; a matrix holding an infinity or NaN gives NaN, without touching the others.  Accuracy is that of fp32
  * products whatever the dtype.  Limits (MMSA_ERR_LIMIT): 2^20 rows or columns, 2^31 values a matrix.
  * scratch: mmsa_orthogonalize_scratch_bytes(...) bytes, 128-byte aligned. */
@@ -470,7 +470,7 @@ MMSA_API int mmsa_orthogonalize(const void* const* src_host, void* const* dst_ho
                                 void* stream);
 /* One Muon step over fp32 matrices:  m += (1 - momentum)(g - m);  u = nesterov ? g + momentum (m - g) : m;
  * p = p (1 - lr weight_decay) - lr sqrt(max(1, rows / cols)) orthogonalize(u).  params and momentum are updated in
- * place, grads are read. */
+ * place (no two of them share memory), grads are read. */
 MMSA_API int mmsa_muon_step(void* const* params_host, const void* const* grads_host, void* const* momentum_host,
                             const int* rows_host, const int* cols_host, int count, double lr, double weight_decay,
                             double momentum, int nesterov, int steps, float eps, void* scratch, void* stream);

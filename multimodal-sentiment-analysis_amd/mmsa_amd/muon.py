@@ -46,8 +46,8 @@ def muon_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], mom
     ``m += (1 - momentum)(g - m);  u = g + momentum (m - g) if nesterov else m;``
     ``p = p (1 - lr weight_decay) - lr sqrt(max(1, rows / cols)) orthogonalize(u)``
 
-    A tensor of more than two dimensions is taken as [first, rest].  The scalars are held by value: a step captured in a
-    HIP graph replays with those of the capture.
+    A tensor of more than two dimensions is taken as [first, rest].  Parameters and momenta are contiguous and no two of
+    them share memory.  The scalars are held by value: a step captured in a HIP graph replays with those of the capture.
     """
     _gpu([*params, *grads, *momenta], "muon_step")
 
@@ -64,7 +64,8 @@ def muon_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], mom
                   nesterov, steps, eps)
     # written through raw pointers: tell autograd (and whoever watches the version counters) that the values changed
     for t in (*params, *momenta):
-        torch.autograd.graph.increment_version(t)
+        if not t.is_inference():
+            torch.autograd.graph.increment_version(t)
 
 
 class Muon(torch.optim.Optimizer):

@@ -71,7 +71,7 @@ def group_norm_act(x: torch.Tensor, num_groups: int, weight=None, bias=None, eps
     if x.dtype not in ops.DTYPE_CODES:
         raise TypeError(f"group_norm_act: float32, bfloat16 or float16 maps, got {x.dtype}")
     B, C = x.shape[:2]
-    ops._group_norm_check(C, num_groups, activation, weight, bias)
+    ops._group_norm_check(C, num_groups, activation, weight, bias, x.device)
     x = _channels_last(x)
     if torch.is_grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad)
                                     or (bias is not None and bias.requires_grad)):

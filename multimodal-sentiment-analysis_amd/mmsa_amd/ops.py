@@ -226,7 +226,7 @@ ACTIVATIONS = {"none": 0, "relu": 1, "silu": 2, "gelu": 3}
 DTYPE_CODES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 
 
-def _group_norm_check(C, groups, act, gamma, beta):
+def _group_norm_check(C, groups, act, gamma, beta, device):
     if act not in ACTIVATIONS:
         raise ValueError(f"group_norm_act: activation {act!r} is none of {', '.join(ACTIVATIONS)}")
     if groups < 1 or C < 1 or C % groups:
@@ -234,6 +234,8 @@ def _group_norm_check(C, groups, act, gamma, beta):
     for t, name in ((gamma, "weight"), (beta, "bias")):
         if t is not None and tuple(t.shape) != (C,):
             raise ValueError(f"group_norm_act: {name} must be [{C}]")
+        if t is not None and t.device != device:
+            raise _lib.MmsaError(f"group_norm_act: {name} lives on {t.device}, the map on {device}")
 
 
 def _group_norm_args(x, gamma, beta, groups, act):
@@ -241,7 +243,7 @@ def _group_norm_args(x, gamma, beta, groups, act):
         raise ValueError("group_norm_act: x must be [B, positions, channels]")
     if x.dtype not in DTYPE_CODES:
         raise TypeError(f"group_norm_act: float32, bfloat16 or float16 maps, got {x.dtype}")
-    _group_norm_check(x.shape[2], groups, act, gamma, beta)
+    _group_norm_check(x.shape[2], groups, act, gamma, beta, x.device)
     return x.shape
 
 
@@ -273,8 +275,8 @@ def group_norm_act_fwd(x, gamma, beta, y, stats, groups: int, eps: float = 1e-5,
     """y = act(group_norm(x) * gamma + beta) over x [B, P, C]; stats [B, groups, 2] float64 <- mean, 1/sqrt(var + eps).
     gamma / beta [C] float32, or None for 1 / 0."""
     B, P, C = _group_norm_args(x, gamma, beta, groups, act)
-    if y.shape != x.shape or tuple(stats.shape) != (B, groups, 2):
-        raise ValueError("group_norm_act_fwd: y like x, stats [B, groups, 2]")
+    if y.shape != x.shape or tuple(stats.shape) != (B, groups, 2) or not x.device == y.device == stats.device:
+        raise ValueError("group_norm_act_fwd: y like x, stats [B, groups, 2], on the device of x")
     if x.numel() == 0:
         return y
     _chk(y, x.dtype, "y"), _chk(stats, torch.float64, "stats"), _chk(x, x.dtype, "x")
@@ -290,6 +292,8 @@ def group_norm_act_bwd(dy, x, gamma, beta, stats, dx, dgamma, dbeta, groups: int
     for t in (dgamma, dbeta):
         if t is not None and tuple(t.shape) != (C,):
             raise ValueError("group_norm_act_bwd: dgamma and dbeta [C]")
+    if any(t is not None and t.device != x.device for t in (dy, stats, dx, dgamma, dbeta)):
+        raise ValueError("group_norm_act_bwd: all operands live on the device of x")
     if x.numel() == 0:
         for t in (dgamma, dbeta):
             if t is not None:
@@ -1142,7 +1146,8 @@ def _ns_scratch(rows, cols, n, device):
 
 
 def orthogonalize(srcs, dsts, steps: int = 5, eps: float = 1e-7):
-    """dsts[i] <- the Newton-Schulz orthogonalisation of srcs[i] ([rows, cols], one dtype for all), in shared launches."""
+    """dsts[i] <- the Newton-Schulz orthogonalisation of srcs[i] ([rows, cols], one dtype for all), in shared launches.
+    dsts[i] may be srcs[i]; apart from that no destination shares memory with another operand."""
     _ns_args(steps, eps)
     if len(srcs) != len(dsts) or any(a.shape != b.shape for a, b in zip(srcs, dsts)):
         raise ValueError("orthogonalize: one destination like every source")
@@ -1162,7 +1167,7 @@ def orthogonalize(srcs, dsts, steps: int = 5, eps: float = 1e-7):
 
 
 def muon_step(params, grads, momenta, lr, weight_decay, momentum, nesterov=True, steps: int = 5, eps: float = 1e-7):
-    """One Muon step over fp32 matrices [rows, cols]; params and momenta are updated in place."""
+    """One Muon step over fp32 matrices [rows, cols]; params and momenta are updated in place (no two share memory)."""
     _ns_args(steps, eps)
     if not len(params) == len(grads) == len(momenta) or any(p.shape != g.shape or p.shape != m.shape
                                                             for p, g, m in zip(params, grads, momenta)):

@@ -327,6 +327,46 @@ def test_more_than_two_to_the_31_values():
     within(y[whole:].view(-1, 4, 16), want[:P - whole], 1024 * U * (1 + want[:P - whole].abs()), torch.bfloat16)
 
 
+@pytest.mark.gpu
+def test_refusals_on_the_gpu():
+    from mmsa_amd import _lib
+    from mmsa_amd.norm import group_norm_act
+    x = torch.zeros(2, 8, 4, device=DEV)
+    with pytest.raises(_lib.MmsaError, match="cpu"):
+        group_norm_act(x, 2, torch.ones(8))
+    with pytest.raises(TypeError):
+        group_norm_act(x.double(), 2)
+    with pytest.raises(TypeError):
+        group_norm_act(x, 2, torch.ones(8, device=DEV, dtype=torch.float16))
+    with pytest.raises(ValueError):
+        group_norm_act(x, 2, torch.ones(16, device=DEV)[::2])
+    for groups in (0, 3, -2):
+        with pytest.raises(ValueError):
+            group_norm_act(x, groups)
+    with pytest.raises(RuntimeError):                    # no gradient of a gradient
+        y = x.clone().requires_grad_()
+        g, = torch.autograd.grad(group_norm_act(y, 2).sum(), y, create_graph=True)
+        g.sum().backward()
+
+
+@pytest.mark.gpu
+def test_a_batch_of_many_tiny_samples_and_one_of_few_long_ones():
+    """The two ends of how a map is cut: 20 000 blocks of one row, and one sample that a whole launch shares."""
+    from mmsa_amd.norm import group_norm_act
+    for size in ((20000, 1, 16, 4), (20000, 3, 6, 2), (1, 300000, 8, 8)):
+        B, P, C, G = size
+        x, w, b, dy = data(B, P, C, torch.bfloat16, seed=C)
+        leaves = [t.detach().requires_grad_() for t in (x.transpose(1, 2), w, b)]
+        y = group_norm_act(leaves[0], G, leaves[1], leaves[2], 1e-5, "relu")
+        got = torch.autograd.grad(y, leaves, dy.transpose(1, 2))
+        want = formula(x.double(), w.double(), b.double(), G, 1e-5, "relu", dy.double())
+        within(y.detach().transpose(1, 2), *want[0], torch.bfloat16)
+        within(got[0].transpose(1, 2), *want[1], torch.bfloat16)
+        # a thread of the long sample sums up to 40 values here, a block up to 512 of those: within the 600 u counted
+        within(got[1], *want[2])
+        within(got[2], *want[3])
+
+
 def test_refusals():
     from mmsa_amd import _lib, ops
     from mmsa_amd.norm import GroupNormAct, group_norm_act
