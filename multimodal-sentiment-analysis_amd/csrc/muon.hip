@@ -737,13 +737,13 @@ __global__ __launch_bounds__(256) void join_kernel(const Group* __restrict__ grp
 
 // ---- matrices that fit one block
 // m <= 64 and n <= 32 * 8 * NT: the whole iteration in one launch, a block of eight waves per matrix.  At these sizes the
-// seventeen dependent launches of the general path are all there is to its time (64 x 288: 72 us).
+// seventeen dependent launches of the general path are all there is to its time (64 x 288, one matrix: 72 us, here 35).
 // X lives in registers: wave w holds the column tiles w, w + 8, ... of 32 columns as the pairs that the product B X
 // takes and gives back -- the accumulator of a product (lane: column; registers: rows 4 h + (e & 3) + 8 (e >> 2) of
 // each 32) is the right operand of the next one with its K index in that order, and the left operand, B, is read from
 // LDS in the same order.  X X^T needs X by rows: a wave turns its tiles over in LDS, and the waves' parts are added up
 // there.  In LDS a pair is one 32-bit word, lo << 16 | hi.
-constexpr int SMALL_M = 64, SMALL_NT = 3, SMALL_N = 256 * SMALL_NT;
+constexpr int SMALL_M = 64;
 constexpr int TURN_ROW = 36, SQUARE_ROW = 68;          // words of a row, padded against bank conflicts
 constexpr int WAVE_WORDS = 3 * 16 * 64;                // a wave's part of X X^T: three of the four 32 x 32 tiles
 static_assert(64 * TURN_ROW <= WAVE_WORDS, "a wave's turning buffer and its part of the sum share their place");
@@ -780,6 +780,13 @@ template <typename V>
 __device__ __forceinline__ V opaque(V v) {
   asm volatile("" : "+v"(v));
   return v;
+}
+
+// orders the LDS accesses of a wave's lanes (the hardware keeps their order, the compiler has to)
+__device__ __forceinline__ void wave_meet() {
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
 }
 
 template <typename T, bool MOM, int NT>
@@ -879,7 +886,7 @@ __global__ __launch_bounds__(512) void small_kernel(const Group gr, float mu, fl
           __builtin_memcpy(&v, p, 4);
           own[row_of(x, e) * TURN_ROW + col] = v;
         }
-      __builtin_amdgcn_wave_barrier();
+      wave_meet();
 #pragma unroll
       for (int g = 0; g < 2; ++g) {
         f16x8 ph[2], pl[2];
@@ -892,7 +899,7 @@ __global__ __launch_bounds__(512) void small_kernel(const Group gr, float mu, fl
         pair_product(ph[1], pl[1], ph[0], pl[0], acc[1], low[1]);
         pair_product(ph[1], pl[1], ph[1], pl[1], acc[2], low[2]);
       }
-      __builtin_amdgcn_wave_barrier();
+      wave_meet();
     }
 #pragma unroll
     for (int k = 0; k < 3; ++k)
@@ -1207,11 +1214,14 @@ int allow_lds(size_t bytes) {
   return MMSA_OK;
 }
 
-bool all_small(const int* rows, const int* cols, int count, int* longest) {
+// Which lists the kernel for small matrices takes, from both sides measured (one matrix, microseconds): 64 x 256 values
+// 29 against 87 for 65 x 256 in the general launches, 64 x 512 44 against 95, 64 x 768 85 against 104.  An optimiser step
+// holds the momentum beside the matrix: 64 x 512 57 against 96, but 64 x 576 103 against 98.
+bool all_small(const int* rows, const int* cols, int count, int widest, int* longest) {
   *longest = 0;
   for (int i = 0; i < count; ++i) {
     const int m = rows[i] < cols[i] ? rows[i] : cols[i], n = rows[i] < cols[i] ? cols[i] : rows[i];
-    if (m > SMALL_M || n > SMALL_N) return false;
+    if (m > SMALL_M || n > widest) return false;
     if (n > *longest) *longest = n;
   }
   return true;
@@ -1235,8 +1245,9 @@ int run_all(const void* const* src, void* const* dst, void* const* mom, const in
     gr.count = count - i0 < GROUP ? count - i0 : GROUP;
     Plan pl;
     make_plan(rows + i0, cols + i0, &gr, &pl);
+    constexpr int NT_MOST = MOM ? 2 : 3;
     int longest;
-    const bool small = all_small(rows + i0, cols + i0, gr.count, &longest);
+    const bool small = all_small(rows + i0, cols + i0, gr.count, 256 * NT_MOST, &longest);
     for (int i = 0; i < gr.count; ++i) {
       Mat& q = gr.mat[i];
       const int at = i0 + pl.from[i];
@@ -1249,7 +1260,7 @@ int run_all(const void* const* src, void* const* dst, void* const* mom, const in
     if (small) {
       const int rc = longest <= 256   ? launch_small<T, MOM, 1>(gr, st, s)
                      : longest <= 512 ? launch_small<T, MOM, 2>(gr, st, s)
-                                      : launch_small<T, MOM, SMALL_NT>(gr, st, s);
+                                      : launch_small<T, MOM, NT_MOST>(gr, st, s);
       if (rc) return rc;
       continue;
     }

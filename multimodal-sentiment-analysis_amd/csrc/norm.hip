@@ -101,7 +101,7 @@ __device__ __forceinline__ float act_fwd(float z) {
 }
 template <int ACT>
 __device__ __forceinline__ float act_slope(float z) {
-  if (ACT == ACT_RELU) return z > 0.f ? 1.f : 0.f;
+  if (ACT == ACT_RELU) return z <= 0.f ? 0.f : 1.f;       // NaN stays NaN
   if (ACT == ACT_SILU) {
     const float s = sigmoid(z);
     return s * fmaf(z, 1.f - s, 1.f);
@@ -405,6 +405,12 @@ struct Channel {
     }
     return act_slope<ACT>(z);
   }
+  // dz of one value; behind a ReLU the gradient is selected, so that no infinity or NaN of dy gets past a closed one
+  template <int ACT>
+  __device__ __forceinline__ float grad(int e, float x, float dy, float& d) const {
+    const float s = slope<ACT>(e, x, d);
+    return ACT == ACT_RELU ? (s != 0.f ? dy : 0.f) : dy * s;
+  }
 };
 
 // per chunk and channel: sum of dz and of dz xhat
@@ -433,7 +439,7 @@ __global__ __launch_bounds__(1024) void gn_bwd_sums_kernel(const T* __restrict__
     for (int e = 0; e < V; ++e) s1[e] = s2[e] = 0.f;
     auto add = [&](int e, float v, float h) {
       float d;
-      const float dz = h * k.template slope<ACT>(e, v, d);
+      const float dz = k.template grad<ACT>(e, v, h, d);
       s1[e] += dz;
       s2[e] = fmaf(dz, d, s2[e]);
     };
@@ -592,7 +598,7 @@ __global__ __launch_bounds__(1024) void gn_bwd_apply_kernel(const T* __restrict_
     }
     auto value = [&](int e, float v, float h) {
       float d;
-      const float dz = h * k.template slope<ACT>(e, v, d);
+      const float dz = k.template grad<ACT>(e, v, h, d);
       return fmaf(k.a[e], dz, -fmaf(d, k2[e], k1[e]));
     };
     p += me.full * hop;           // backwards, as in the forward pass
@@ -861,7 +867,7 @@ __global__ __launch_bounds__(1024) void gn_slab_bwd_kernel(const T* __restrict__
 #pragma unroll
       for (int e = 0; e < W; ++e) {
         float d;
-        const float dz = g[e] * ch.template slope<ACT>(e, v[e], d);
+        const float dz = ch.template grad<ACT>(e, v[e], g[e], d);
         s1[e] += dz;
         s2[e] = fmaf(dz, d, s2[e]);
       }
@@ -939,7 +945,7 @@ __global__ __launch_bounds__(1024) void gn_slab_bwd_kernel(const T* __restrict__
 #pragma unroll
       for (int e = 0; e < W; ++e) {
         float d;
-        const float dz = gr[e] * ch.template slope<ACT>(e, v[e], d);
+        const float dz = ch.template grad<ACT>(e, v[e], gr[e], d);
         v[e] = fmaf(ch.a[e], dz, -fmaf(d, k2, k1));
       }
       f[k].set(v);

@@ -32,9 +32,7 @@ def orthogonalize(matrices: Union[torch.Tensor, Sequence[torch.Tensor]], steps: 
     ms = [matrices] if single else list(matrices)
     _gpu(ms, "orthogonalize")
     with torch.no_grad():
-        srcs = [m.detach().contiguous() for m in ms]
-        dsts = [torch.empty_like(m) for m in srcs]
-        ops.orthogonalize(srcs, dsts, steps, eps)
+        dsts = ops.orthogonalize([m if m.is_contiguous() else m.contiguous() for m in ms], None, steps, eps)
     return dsts[0] if single else dsts
 
 
@@ -49,23 +47,10 @@ def muon_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], mom
     A tensor of more than two dimensions is taken as [first, rest].  Parameters and momenta are contiguous and no two of
     them share memory.  The scalars are held by value: a step captured in a HIP graph replays with those of the capture.
     """
-    _gpu([*params, *grads, *momenta], "muon_step")
-
-    def flat(ts, name):
-        out = []
-        for t in ts:
-            if t.dim() < 2 or not t.is_contiguous():
-                raise ValueError(f"muon_step: {name} must be contiguous and have at least two dimensions")
-            out.append(t.detach().view(t.shape[0], -1))
-        return out
-
-    grads = [g.contiguous() for g in grads]
-    ops.muon_step(flat(params, "params"), flat(grads, "grads"), flat(momenta, "momenta"), lr, weight_decay, momentum,
-                  nesterov, steps, eps)
+    ops.muon_step(params, [g if g.is_contiguous() else g.contiguous() for g in grads], momenta, lr, weight_decay,
+                  momentum, nesterov, steps, eps)
     # written through raw pointers: tell autograd (and whoever watches the version counters) that the values changed
-    for t in (*params, *momenta):
-        if not t.is_inference():
-            torch.autograd.graph.increment_version(t)
+    torch.autograd.graph.increment_version([t for t in (*params, *momenta) if not t.is_inference()])
 
 
 class Muon(torch.optim.Optimizer):

@@ -1126,12 +1126,22 @@ def scalar_axpy(dst, a, b, alpha):
 
 # ------------------------------------------------------------------------------------------- orthogonalised updates
 def _matrices(ts, dtype, name):
+    """Addresses of non-empty contiguous tensors of one device, each taken as [first, rest]."""
+    ptrs = []
+    device = ts[0].get_device()
     for t in ts:
-        if t.dim() != 2 or t.numel() == 0:
-            raise ValueError(f"{name}: non-empty matrices [rows, cols], got {tuple(t.shape)}")
-    if len({t.device for t in ts}) > 1:
-        raise ValueError(f"{name}: the matrices of one call live on one device")
-    return _parr([_chk(t, dtype, name) for t in ts])
+        if t.dim() < 2 or not t.numel():
+            raise ValueError(f"{name}: non-empty, of at least two dimensions, got {tuple(t.shape)}")
+        ptrs.append(_chk(t, dtype, name))
+        if _OPERANDS.dev != device:
+            raise ValueError(f"{name}: the matrices of one call live on one device")
+    return ptrs
+
+
+def _sizes(ts):
+    n = len(ts)
+    rows = [t.shape[0] for t in ts]
+    return (ctypes.c_int * n)(*rows), (ctypes.c_int * n)(*[t.numel() // r for t, r in zip(ts, rows)])
 
 
 def _ns_args(steps, eps):
@@ -1145,29 +1155,39 @@ def _ns_scratch(rows, cols, n, device):
     return torch.empty((_lib.query("mmsa_orthogonalize_scratch_bytes", rows, cols, n),), dtype=torch.uint8, device=device)
 
 
-def orthogonalize(srcs, dsts, steps: int = 5, eps: float = 1e-7):
+def orthogonalize(srcs, dsts=None, steps: int = 5, eps: float = 1e-7):
     """dsts[i] <- the Newton-Schulz orthogonalisation of srcs[i] ([rows, cols], one dtype for all), in shared launches.
-    dsts[i] may be srcs[i]; apart from that no destination shares memory with another operand."""
+    dsts[i] may be srcs[i]; apart from that no destination shares memory with another operand.  Without ``dsts`` new
+    tensors are made.  Returns the destinations."""
     _ns_args(steps, eps)
-    if len(srcs) != len(dsts) or any(a.shape != b.shape for a, b in zip(srcs, dsts)):
+    if dsts is not None and (len(srcs) != len(dsts) or any(a.shape != b.shape for a, b in zip(srcs, dsts))):
         raise ValueError("orthogonalize: one destination like every source")
     if not srcs:
-        return
+        return []
     dtype = srcs[0].dtype
     if dtype not in DTYPE_CODES:
         raise TypeError(f"orthogonalize: float32, bfloat16 or float16 matrices, got {dtype}")
+    if any(t.dim() != 2 for t in srcs):
+        raise ValueError("orthogonalize: matrices [rows, cols]")
     n = len(srcs)
-    src, dst = _matrices(srcs, dtype, "orthogonalize"), _matrices(dsts, dtype, "orthogonalize")
-    if dsts[0].device != srcs[0].device:
-        raise ValueError("orthogonalize: the matrices of one call live on one device")
-    rows, cols = _iarr([t.shape[0] for t in srcs]), _iarr([t.shape[1] for t in srcs])
+    src = _matrices(srcs, dtype, "orthogonalize")
+    if dsts is None:
+        dsts = [torch.empty_like(t) for t in srcs]
+        dst = [t.data_ptr() for t in dsts]
+    else:
+        dst = _matrices(dsts, dtype, "orthogonalize")
+        if dsts[0].device != srcs[0].device:
+            raise ValueError("orthogonalize: the matrices of one call live on one device")
+    rows, cols = _sizes(srcs)
     stream = _stream()
-    _lib.call("mmsa_orthogonalize", src, dst, rows, cols, n, DTYPE_CODES[dtype], int(steps), eps,
+    _lib.call("mmsa_orthogonalize", _parr(src), _parr(dst), rows, cols, n, DTYPE_CODES[dtype], int(steps), eps,
               _ns_scratch(rows, cols, n, srcs[0].device).data_ptr(), stream)
+    return dsts
 
 
 def muon_step(params, grads, momenta, lr, weight_decay, momentum, nesterov=True, steps: int = 5, eps: float = 1e-7):
-    """One Muon step over fp32 matrices [rows, cols]; params and momenta are updated in place (no two share memory)."""
+    """One Muon step over contiguous fp32 tensors, each taken as a matrix [first, rest]; params and momenta are updated in
+    place (no two share memory)."""
     _ns_args(steps, eps)
     if not len(params) == len(grads) == len(momenta) or any(p.shape != g.shape or p.shape != m.shape
                                                             for p, g, m in zip(params, grads, momenta)):
@@ -1178,9 +1198,10 @@ def muon_step(params, grads, momenta, lr, weight_decay, momentum, nesterov=True,
     ptrs = [_matrices(ts, F32, name) for ts, name in ((params, "params"), (grads, "grads"), (momenta, "momenta"))]
     if not params[0].device == grads[0].device == momenta[0].device:
         raise ValueError("muon_step: the matrices of one call live on one device")
-    if len(set(ptrs[0]) | set(ptrs[2])) != 2 * n or set(ptrs[1]) & (set(ptrs[0]) | set(ptrs[2])):
+    written = {*ptrs[0], *ptrs[2]}
+    if len(written) != 2 * n or not written.isdisjoint(ptrs[1]):
         raise ValueError("muon_step: a parameter or momentum buffer is listed twice")
-    rows, cols = _iarr([t.shape[0] for t in params]), _iarr([t.shape[1] for t in params])
+    rows, cols = _sizes(params)
     stream = _stream()
-    _lib.call("mmsa_muon_step", *ptrs, rows, cols, n, float(lr), float(weight_decay), float(momentum), int(nesterov),
+    _lib.call("mmsa_muon_step", *map(_parr, ptrs), rows, cols, n, float(lr), float(weight_decay), float(momentum), int(nesterov),
               int(steps), eps, _ns_scratch(rows, cols, n, params[0].device).data_ptr(), stream)

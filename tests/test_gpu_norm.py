@@ -328,6 +328,23 @@ def test_more_than_two_to_the_31_values():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("size", [(3, 6, 8, 4), (2, 4096, 64, 2)])          # in registers, and cut
+@pytest.mark.parametrize("bad", [float("inf"), float("nan")])
+def test_a_closed_relu_lets_no_infinity_or_nan_of_dy_through(size, bad):
+    from mmsa_amd.norm import group_norm_act
+    B, P, C, G = size
+    x, w, b, dy = data(B, P, C, torch.float32, seed=5)
+    leaves = [t.detach().requires_grad_() for t in (x.transpose(1, 2), w, b)]
+    y = group_norm_act(leaves[0], G, leaves[1], leaves[2], 1e-5, "relu")
+    clean = torch.where(y.detach() > 0, dy.transpose(1, 2), 0.0)
+    dirty = torch.where(y.detach() > 0, dy.transpose(1, 2), bad)
+    want = torch.autograd.grad(y, leaves, clean, retain_graph=True)
+    got = torch.autograd.grad(y, leaves, dirty)
+    for g, v in zip(got, want):
+        assert torch.equal(g, v)
+
+
+@pytest.mark.gpu
 def test_refusals_on_the_gpu():
     from mmsa_amd import _lib
     from mmsa_amd.norm import group_norm_act
