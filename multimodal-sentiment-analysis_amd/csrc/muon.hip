@@ -374,7 +374,7 @@ __device__ __forceinline__ void multiply(f32x16 (&acc)[Tile<BT>::W][Tile<BT>::W]
         for (int e = 0; e < 16; ++e) low[x][y][e] = 0.f;
   }
   constexpr int W = S::W, G = S::G, ROW = S::ROW, OPER = S::OPER, LOADS = S::LOADS;
-  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+  const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);     // LDS places in scalars
   const int nk = nk32 * 2 / G;
   // a wave's load fills 16 / G rows
   const int lrow = lane / (4 * G), lu = lane % (4 * G);
@@ -803,7 +803,6 @@ __global__ __launch_bounds__(512) void small_kernel(const Group gr, float mu, fl
   // element e of row tile x of column tile t: row i, column j, and its place in the caller's matrix (0 behind the edges,
   // so that every load can be issued without a branch: a branch would wait for each in turn)
   auto row_of = [&](int x, int e) { return x * 32 + (e & 3) + 8 * (e >> 2) + 4 * half; };
-  auto col_of = [&](int t) { return (t * 8 + w) * 32 + col; };
   const unsigned si = tall ? 1 : q.cols, sj = tall ? q.cols : 1;
   unsigned corner = 4 * half * si + (w * 32 + col) * sj;
   int below = q.m - 4 * half, right = q.n - w * 32 - col;      // rows and columns there are from the corner on
