@@ -164,11 +164,14 @@ template <typename T, bool ONCE>
 __global__ __launch_bounds__(1024) void gn_stats_kernel(const T* __restrict__ x, const Cut cut,
                                                         double* __restrict__ part) {
   constexpr int V = Io<T>::V, U = 4;            // U loads in flight per thread
-  extern __shared__ float sh[];                 // [3][slots]: mean, M2, count of every (thread, element)
+  extern __shared__ float sh[];                 // [3][slots]: mean, M2, count of every slot
   const int tid = threadIdx.x;
   const long b = blockIdx.x / cut.nchunk, ch = blockIdx.x % cut.nchunk;
   const T* xs = x + b * cut.S;
-  const int slots = cut.columns == 1 ? cut.active * V : cut.period * V;
+  // a slot is a value of a thread's vectors, or all V of them where they belong to one group
+  const bool whole = cut.Cg % V == 0;
+  const int each = whole ? V : 1, C = cut.C / each, Cg = cut.Cg / each;
+  const int slots = (cut.columns == 1 ? cut.active * V : cut.period * V) / each;
   float* smean = sh;
   float* sm2 = sh + slots;
   float* scnt = sh + 2 * slots;
@@ -220,6 +223,7 @@ __global__ __launch_bounds__(1024) void gn_stats_kernel(const T* __restrict__ x,
         q[e] = fmaf(d, d, q[e]);
       }
     }
+    float n[V];
 #pragma unroll
     for (int e = 0; e < V; ++e) {
       if (e < me.rest) {
@@ -229,24 +233,48 @@ __global__ __launch_bounds__(1024) void gn_stats_kernel(const T* __restrict__ x,
         s[e] += d;
         q[e] = fmaf(d, d, q[e]);
       }
-      const float n = (float)(me.full + (e < me.rest ? 1 : 0));
-      const float m = n > 0.f ? s[e] / n : 0.f;
-      smean[t * V + e] = k[e] + m;
-      sm2[t * V + e] = fmaxf(fmaf(-s[e], m, q[e]), 0.f);
-      scnt[t * V + e] = n;
+      n[e] = (float)(me.full + (e < me.rest ? 1 : 0));
+      const float m = n[e] > 0.f ? s[e] / n[e] : 0.f;
+      q[e] = fmaxf(fmaf(-s[e], m, q[e]), 0.f);
+      s[e] = m;                                 // now the mean and M2 about it, k being the origin
+    }
+    if (whole) {                                // (a short vector leaves whole groups' values out at its end)
+      float count = 0.f, sum = 0.f, m2 = 0.f;
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        s[e] += k[e] - k[0];
+        count += n[e];
+        sum = fmaf(n[e], s[e], sum);
+      }
+      const float m = count > 0.f ? sum / count : 0.f;
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        const float d = s[e] - m;
+        m2 += n[e] > 0.f ? fmaf(n[e] * d, d, q[e]) : 0.f;
+      }
+      smean[t] = k[0] + m;
+      sm2[t] = m2;
+      scnt[t] = count;
+    } else {
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        smean[t * V + e] = k[e] + s[e];
+        sm2[t * V + e] = q[e];
+        scnt[t * V + e] = n[e];
+      }
     }
   }
   __syncthreads();
-  // a team of lanes per group, all groups at once where there are enough threads; slot q belongs to channel q % C
-  // (slots is a multiple of C)
-  const int per = slots / cut.C * cut.Cg;
+  // a team of lanes per group, all groups at once where there are enough threads; slot q belongs to channel
+  // (or V channels) q % C (slots is a multiple of C)
+  const int per = slots / C * Cg;
   const int lane = tid & (cut.team - 1), teams = blockDim.x / cut.team;
   for (int g0 = 0; g0 < cut.G; g0 += teams) {          // uniform: all lanes take part in the sums
     const int g = g0 + tid / cut.team;
     const bool mine = g < cut.G;
     double n = 0.0, sum = 0.0;
     for (int i = lane; mine && i < per; i += cut.team) {
-      const int q = (i / cut.Cg) * cut.C + g * cut.Cg + i % cut.Cg;
+      const int q = (i / Cg) * C + g * Cg + i % Cg;
       n += (double)scnt[q];
       sum += (double)scnt[q] * (double)smean[q];
     }
@@ -255,7 +283,7 @@ __global__ __launch_bounds__(1024) void gn_stats_kernel(const T* __restrict__ x,
     const double mean = n > 0.0 ? sum / n : 0.0;
     double m2 = 0.0;
     for (int i = lane; mine && i < per; i += cut.team) {
-      const int q = (i / cut.Cg) * cut.C + g * cut.Cg + i % cut.Cg;
+      const int q = (i / Cg) * C + g * Cg + i % Cg;
       const double d = (double)smean[q] - mean;
       if (scnt[q] > 0.f) m2 += (double)sm2[q] + (double)scnt[q] * d * d;
     }
@@ -492,31 +520,69 @@ __global__ __launch_bounds__(1024) void gn_bwd_sums_kernel(const T* __restrict__
   }
 }
 
-// joins the chunks of one (sample, group): channel sums [b][c][2], and the two means of the group over N values
-__global__ __launch_bounds__(256) void gn_bwd_join_kernel(const float* __restrict__ part, const Cut cut,
-                                                          const float* __restrict__ gamma, float* __restrict__ sums,
-                                                          float* __restrict__ coef) {
-  __shared__ double red[16];
-  const long b = blockIdx.x / cut.G;
-  const int g = blockIdx.x % cut.G, lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-  double c1 = 0.0, c2 = 0.0;
-  for (int j = w; j < cut.Cg; j += 4) {           // one wave per channel
-    const int c = g * cut.Cg + j;
+// Joins the chunks: channel sums [b][c][2].  A block has up to 64 channels of a sample, a channel per lane, the chunks
+// shared out among its waves and joined in order.  Where a block's channels are whole groups (`span` = 64 / Cg * Cg) it
+// also leaves the two means of each over N values; larger groups are joined by the kernel behind this one.
+__global__ __launch_bounds__(1024) void gn_bwd_join_kernel(const float* __restrict__ part, const Cut cut, int span,
+                                                           const float* __restrict__ gamma, float* __restrict__ sums,
+                                                           float* __restrict__ coef) {
+  __shared__ double red[16][64][2];
+  const int blocks = (cut.C + span - 1) / span;
+  const long b = blockIdx.x / blocks;
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, nw = blockDim.x >> 6;
+  const int c0 = blockIdx.x % blocks * span, c = c0 + lane;
+  const bool mine = lane < span && c < cut.C;
+  double a = 0.0, q = 0.0;
+  if (mine) {
     const float* p = part + (b * cut.nchunk * cut.C + c) * 2;
-    double a = 0.0, q = 0.0;
-    for (long i = lane; i < cut.nchunk; i += 64) {
+#pragma unroll 4
+    for (long i = w; i < cut.nchunk; i += nw) {
       a += (double)p[i * cut.C * 2];
       q += (double)p[i * cut.C * 2 + 1];
     }
-    a = wave_sum_d(a);
-    q = wave_sum_d(q);
-    if (lane == 0) {
-      sums[(b * cut.C + c) * 2] = (float)a;
-      sums[(b * cut.C + c) * 2 + 1] = (float)q;
-      const double gm = gamma ? (double)gamma[c] : 1.0;
-      c1 += a * gm;
-      c2 += q * gm;
+  }
+  red[w][lane][0] = a;
+  red[w][lane][1] = q;
+  __syncthreads();
+  if (w) return;
+  for (int k = 1; k < nw; ++k) {
+    a += red[k][lane][0];
+    q += red[k][lane][1];
+  }
+  if (mine) {
+    sums[(b * cut.C + c) * 2] = (float)a;
+    sums[(b * cut.C + c) * 2 + 1] = (float)q;
+  }
+  if (cut.Cg > 64) return;
+  const double gm = mine && gamma ? (double)gamma[c] : 1.0;
+  red[0][lane][0] = a * gm;
+  red[0][lane][1] = q * gm;
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  if (lane < span / cut.Cg && c0 + lane * cut.Cg < cut.C) {
+    double c1 = 0.0, c2 = 0.0;
+    for (int i = lane * cut.Cg; i < (lane + 1) * cut.Cg; ++i) {
+      c1 += red[0][i][0];
+      c2 += red[0][i][1];
     }
+    const double n = (double)(cut.S / cut.C) * cut.Cg;
+    float* o = coef + 2 * (b * cut.G + c0 / cut.Cg + lane);
+    o[0] = (float)(c1 / n);
+    o[1] = (float)(c2 / n);
+  }
+}
+
+// the two means of a group of more than 64 channels from their sums
+__global__ __launch_bounds__(256) void gn_bwd_coef_kernel(const float* __restrict__ sums, const Cut cut,
+                                                          const float* __restrict__ gamma, float* __restrict__ coef) {
+  __shared__ double red[16];
+  const long b = blockIdx.x / cut.G;
+  const int c0 = blockIdx.x % cut.G * cut.Cg;
+  double c1 = 0.0, c2 = 0.0;
+  for (int c = c0 + threadIdx.x; c < c0 + cut.Cg; c += 256) {
+    const double gm = gamma ? (double)gamma[c] : 1.0;
+    c1 += (double)sums[(b * cut.C + c) * 2] * gm;
+    c2 += (double)sums[(b * cut.C + c) * 2 + 1] * gm;
   }
   c1 = block_sum_d(c1, red);
   c2 = block_sum_d(c2, red);
@@ -883,10 +949,12 @@ __global__ __launch_bounds__(1024) void gn_slab_bwd_kernel(const T* __restrict__
     }
   }
   __syncthreads();
-  const int nseg = (int)blockDim.x / p.L > 1 ? (int)blockDim.x / p.L : 1;
+  // two stages of at most 32 additions one after another: more segments would leave their sum to a few threads
+  const int spare = (int)blockDim.x / p.L, nseg = spare > 32 ? 32 : spare > 1 ? spare : 1;
   for (int i = tid; i < p.L * nseg; i += blockDim.x) {
     const int c = i % p.L;
     float a = 0.f, t = 0.f;
+#pragma unroll 4
     for (int r = i / p.L; r < q.rp; r += nseg) {
       a += sh[(r * Lf + c) * 2];
       t += sh[(r * Lf + c) * 2 + 1];
@@ -897,6 +965,7 @@ __global__ __launch_bounds__(1024) void gn_slab_bwd_kernel(const T* __restrict__
   __syncthreads();
   for (int c = tid; c < p.L; c += blockDim.x) {
     float a = 0.f, t = 0.f;
+#pragma unroll 4
     for (int i = c; i < p.L * nseg; i += p.L) {
       a += seg[2 * i];
       t += seg[2 * i + 1];
@@ -994,6 +1063,10 @@ bool make_cut(long batch, long positions, int C, int G, int dtype, Cut* cut) {
   // block's prologue and the joining of its sums cost about as much as four)
   long iters = (rows * batch + 1023) / 1024;
   if (iters < 8) iters = 8;
+  // of wide maps at least 32 positions as long as that leaves a block for every compute unit: a chunk's sums are two
+  // floats a channel, written and read again
+  const long deep = 32l * C / ((long)V * cut->row);
+  if (iters < deep) iters = deep < rows * batch / 256 ? deep : iters > rows * batch / 256 ? iters : rows * batch / 256;
   if (iters > rows) iters = rows;
   cut->iters = (int)iters;
   cut->nchunk = (rows + iters - 1) / iters;
@@ -1020,8 +1093,24 @@ int allow_lds(size_t bytes) {
   return MMSA_OK;
 }
 
-// Whether a pass can keep its slabs in registers, and how.  `most`: registers of 4 bytes a thread may hold of one map.
-bool make_slab(long batch, long positions, int C, int G, int dtype, int most, Slab* q) {
+// What a pass costs in microseconds either way, from measurements over 1 to 64 samples of 256 to 8192 positions of 61 to
+// 512 channels.  In registers: a block walks its P rows of `row` bytes at a pace of its own, and beyond 256 blocks they
+// wait for each other; narrow rows cost nearly what wide ones do (64 samples of 8192 positions in 32 groups of 2 bf16
+// channels: 176 us against 50 cut in chunks, backward 264 against 72; 16 samples of 4096 in groups of 16: 38 against 55).
+// In chunks: the launches, and the bytes of all passes.
+float slab_cost(const Slab& q, int dtype, bool backward) {
+  const int size = dtype == 0 ? 4 : 2, row = q.bundle * q.Cg * size;
+  const float blocks = (float)q.batch * q.bundles / 256.f, rounds = blocks > 1.f ? blocks : 1.f;
+  return backward ? 10.f + 1e-3f * q.P * rounds * (3.f + (size == 4 ? .14f : .2f) * row)
+                  : 6.f + 1e-3f * q.P * rounds * (2.4f + (size == 4 ? .05f : .0875f) * row);
+}
+float cut_cost(const Slab& q, int dtype, bool backward) {
+  const float mb = 1e-6f * q.batch * q.S * (dtype == 0 ? 4 : 2);
+  return backward ? (dtype == 0 ? 17.f + .75f * mb : 21.f + .8f * mb) : (dtype == 0 ? 14.f + .45f * mb : 18.f + .52f * mb);
+}
+
+// Whether a pass keeps its slabs in registers, and how.  `most`: registers of 4 bytes a thread may hold of one map.
+bool make_slab(long batch, long positions, int C, int G, int dtype, int most, bool backward, Slab* q) {
   const int size = dtype == 0 ? 4 : 2, Cg = C / G;
   if (positions > 65536) return false;
   q->S = positions * C;
@@ -1050,7 +1139,8 @@ bool make_slab(long batch, long positions, int C, int G, int dtype, int most, Sl
       q->threads = t;
       q->vecs = (q->P + q->rp - 1) / q->rp;
       const int cap = t < 1024 ? 4 : most / reg < 16 ? most / reg : 16;
-      if (q->vecs <= cap) return batch * q->bundles <= GN_MAX_BLOCKS;
+      if (q->vecs <= cap)
+        return batch * q->bundles <= GN_MAX_BLOCKS && slab_cost(*q, dtype, backward) <= cut_cost(*q, dtype, backward);
     }
   }
   return false;
@@ -1126,7 +1216,7 @@ template <typename T>
 int gn_fwd(const void* x, const float* gamma, const float* beta, void* y, double* stats, void* scratch, long batch,
            const Cut& cut, int dtype, float eps, int act, hipStream_t s) {
   Slab q;
-  if (make_slab(batch, cut.S / cut.C, cut.C, cut.G, dtype, FWD_REGS, &q)) {
+  if (make_slab(batch, cut.S / cut.C, cut.C, cut.G, dtype, FWD_REGS, false, &q)) {
     if (q.W == Io<T>::V) return slab_fwd_n<T, Io<T>::V>(x, gamma, beta, y, stats, eps, act, q, s);
     if constexpr (sizeof(T) == 2)
       if (q.W == 4) return slab_fwd_n<T, 4>(x, gamma, beta, y, stats, eps, act, q, s);
@@ -1151,7 +1241,11 @@ int cut_bwd(const T* dy, const T* x, const float* gamma, const float* beta, cons
   const size_t lds = 2 * sizeof(float) * slots_of(cut, dtype);
   if (int rc = allow_lds<gn_bwd_sums_kernel<T, ACT, ONCE>>(lds)) return rc;
   hipLaunchKernelGGL((gn_bwd_sums_kernel<T, ACT, ONCE>), grid, block, lds, s, dy, x, gamma, beta, stats, cut, part);
-  hipLaunchKernelGGL(gn_bwd_join_kernel, dim3((unsigned)(batch * cut.G)), dim3(256), 0, s, part, cut, gamma, sums, coef);
+  const int span = cut.Cg > 64 ? 64 : 64 / cut.Cg * cut.Cg;
+  hipLaunchKernelGGL(gn_bwd_join_kernel, dim3((unsigned)(batch * mmsa_cdiv(cut.C, span))),
+                     dim3(cut.nchunk < 64 ? 256 : 1024), 0, s, part, cut, span, gamma, sums, coef);
+  if (cut.Cg > 64 && dx)
+    hipLaunchKernelGGL(gn_bwd_coef_kernel, dim3((unsigned)(batch * cut.G)), dim3(256), 0, s, sums, cut, gamma, coef);
   const int nparam = dgamma || dbeta ? mmsa_cdiv(cut.C, 64) : 0;
   const unsigned blocks = nparam + (dx ? grid.x : 0);
   if (blocks)
@@ -1165,7 +1259,7 @@ int gn_bwd(const void* dy, const void* x, const float* gamma, const float* beta,
            float* dgamma, float* dbeta, void* scratch, long batch, const Cut& cut, int dtype, hipStream_t s) {
   float* part = static_cast<float*>(scratch);
   Slab q;
-  if (make_slab(batch, cut.S / cut.C, cut.C, cut.G, dtype, BWD_REGS, &q)) {
+  if (make_slab(batch, cut.S / cut.C, cut.C, cut.G, dtype, BWD_REGS, true, &q)) {
     if (q.W == Io<T>::V)
       return slab_bwd_n<T, Io<T>::V, ACT>(dy, x, gamma, beta, stats, dx, dgamma, dbeta, part, q, s);
     if constexpr (sizeof(T) == 2)
@@ -1201,7 +1295,9 @@ int gn_bwd_act(int act, const void* dy, const void* x, const float* gamma, const
 int check_size(long batch, long positions, int channels, int groups, int dtype, Cut* cut) {
   if (!make_cut(batch, positions, channels, groups, dtype, cut)) return MMSA_ERR_ARG;
   if (channels > GN_MAX_CHANNELS || slots_of(*cut, dtype) > GN_MAX_SLOTS) return MMSA_ERR_LIMIT;
-  if (batch > GN_MAX_BLOCKS / cut->nchunk || batch > 4 * GN_MAX_BLOCKS / groups) return MMSA_ERR_LIMIT;
+  // the joining kernels have a block of at most 256 threads per group, or per 64 channels (1024 only beside many chunks)
+  const int most = groups > mmsa_cdiv(channels, 64) ? groups : mmsa_cdiv(channels, 64);
+  if (batch > GN_MAX_BLOCKS / cut->nchunk || batch > 4 * GN_MAX_BLOCKS / most) return MMSA_ERR_LIMIT;
   return MMSA_OK;
 }
 

@@ -367,6 +367,26 @@ def test_refusals_on_the_gpu():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("size", [(2, 1500, 256, 1), (2, 1500, 260, 2), (3, 700, 195, 3), (2, 4096, 64, 32),
+                                  (40, 600, 66, 33), (1, 9000, 1024, 8), (5, 300, 128, 2)])
+def test_groups_of_many_and_of_two_channels(size, dtype):
+    """More than 64 channels a group, groups that are no multiple of 64 or of a vector, and groups of two channels over
+    many positions: the ways in which the sums of chunks are joined."""
+    from mmsa_amd.norm import group_norm_act
+    B, P, C, G = size
+    x, w, b, dy = data(B, P, C, dtype, seed=C)
+    leaves = [t.detach().requires_grad_() for t in (x.transpose(1, 2), w, b)]
+    y = group_norm_act(leaves[0], G, leaves[1], leaves[2], 1e-5, "silu")
+    got = torch.autograd.grad(y, leaves, dy.transpose(1, 2))
+    want = formula(x.double(), w.double(), b.double(), G, 1e-5, "silu", dy.double())
+    within(y.detach().transpose(1, 2), *want[0], dtype)
+    within(got[0].transpose(1, 2), *want[1], dtype)
+    within(got[1], *want[2])
+    within(got[2], *want[3])
+
+
+@pytest.mark.gpu
 def test_a_batch_of_many_tiny_samples_and_one_of_few_long_ones():
     """The two ends of how a map is cut: 20 000 blocks of one row, and one sample that a whole launch shares."""
     from mmsa_amd.norm import group_norm_act
