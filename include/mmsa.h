@@ -438,7 +438,8 @@ MMSA_API int mmsa_copy_multi(const void* const* srcs, void* const* dsts, const l
  * each may be null (1 / 0); stats [batch][groups][2] doubles (mean, 1 / sqrt(var + eps)), written by the forward pass
  * and read by the backward pass.  act: MMSA_ACT_*.  dx, dgamma, dbeta may each be null (not wanted).  Results do not
  * depend on the order in which workgroups run.  Limits (MMSA_ERR_LIMIT): 4096 channels; where the channels are no
- * multiple of a 16-byte vector, channels * (values per vector) / gcd at most 12288; 4 million samples.
+ * multiple of a 16-byte vector, channels * (values per vector) / gcd at most 12288; 4 million samples, 16 million
+ * groups or runs of 64 channels over all samples.
  * scratch: mmsa_group_norm_act_scratch_bytes(...) bytes, 8-byte aligned. */
 #define MMSA_F32 0
 #define MMSA_BF16 1
@@ -460,9 +461,10 @@ MMSA_API int mmsa_group_norm_act_bwd(const void* dy, const void* x, const float*
  * dst = X_steps of  X_0 = src / max(||src||_F, eps),  X <- (a I + b S + c S S) X,  S = X X^T  (on src^T where src has
  * more rows than columns), (a, b, c) = (3.4445, -4.775, 2.0315): singular values are driven towards 1.  `count`
  * matrices of one dtype (MMSA_F32 / MMSA_BF16 / MMSA_F16), row-major contiguous [rows][cols], in shared launches;
- * dst[i] may be src[i], apart from that no destination shares memory with another operand.  *_host: host arrays of `count` device pointers / sizes.  1 <= steps <= 16.  A zero matrix
- * gives zeros; a matrix holding an infinity or NaN gives NaN, without touching the others.  Accuracy is that of fp32
- * products whatever the dtype.  Limits (MMSA_ERR_LIMIT): 2^20 rows or columns, 2^31 values a matrix.
+ * dst[i] may be src[i], apart from that no destination shares memory with another operand.  *_host: host arrays of
+ * `count` device pointers / sizes.  1 <= steps <= 16.  A zero matrix gives zeros; a matrix holding an infinity or NaN
+ * gives NaN, without touching the others.  Accuracy is that of fp32 products whatever the dtype.  Limits
+ * (MMSA_ERR_LIMIT): 2^20 rows or columns, 2^31 values a matrix.
  * scratch: mmsa_orthogonalize_scratch_bytes(...) bytes, 128-byte aligned. */
 MMSA_API long mmsa_orthogonalize_scratch_bytes(const int* rows_host, const int* cols_host, int count);
 MMSA_API int mmsa_orthogonalize(const void* const* src_host, void* const* dst_host, const int* rows_host,

@@ -159,7 +159,10 @@ __device__ __forceinline__ Share share_of(const Cut& cut, long ch, int t) {
 // is.  Threads, chunks and channels are then joined in 64 bits by the parallel-variance formula
 //   M2 = sum M2_i + sum n_i (mean_i - mean)^2.
 // ONCE: the map is larger than what the last-level cache would keep for the next pass; reading it past that cache spares
-// the eviction of dirty lines (268 MB: 52 us instead of 80).
+// the eviction of dirty lines (268 MB: 49 us instead of 80, 5.5 TB/s; at 128 MB the two ways are within 5 %).
+// Bound by memory: a map is read once here and once by the pass behind.  Four loads in flight per thread, four blocks of
+// 256 threads a compute unit.  The joining afterwards took most of the time of a short chunk while a group's slots were
+// added up one after another: hence teams of lanes per group, and one slot for a whole vector.
 template <typename T, bool ONCE>
 __global__ __launch_bounds__(1024) void gn_stats_kernel(const T* __restrict__ x, const Cut cut,
                                                         double* __restrict__ part) {
@@ -325,6 +328,9 @@ __global__ __launch_bounds__(64) void gn_stats_join_kernel(const double* __restr
 }
 
 // ---------------------------------------------------------------------------------------------------- forward map
+// y = act((x - mean) a + beta), a = gamma rstd.  Bound by memory: 8 x 65536 x 256 bf16 with SiLU 94 us, 537 MB at
+// 5.7 TB/s.  Blocks and threads go through the map in the opposite order of the statistics pass, so that what that pass
+// read last is taken from the last-level cache (4 x 16384 x 512 bf16: 29 us, behind statistics of 25 us).
 template <typename T, int ACT, bool ONCE>
 __global__ __launch_bounds__(1024) void gn_apply_kernel(const T* __restrict__ x, const float* __restrict__ gamma,
                                                         const float* __restrict__ beta,
@@ -441,7 +447,9 @@ struct Channel {
   }
 };
 
-// per chunk and channel: sum of dz and of dz xhat
+// Per chunk and channel: sum of dz and of dz xhat (rstd is one factor, applied at the end).  A thread sums 32 to 64 rows
+// in 32 bits, the block joins its threads, the chunks are joined in 64 bits.  4 x 16384 x 512 bf16, SiLU: 31 us, 134 MB at
+// 4.3 TB/s; the vector unit is as busy as memory (the slope of an activation is 12 to 20 instructions a value).
 template <typename T, int ACT, bool ONCE>
 __global__ __launch_bounds__(1024) void gn_bwd_sums_kernel(const T* __restrict__ dy, const T* __restrict__ x,
                                                            const float* __restrict__ gamma,
@@ -622,7 +630,8 @@ __global__ __launch_bounds__(1024) void gn_param_kernel(const float* __restrict_
   param_sums(sums, batch, C, blockIdx.x * 64, dgamma, dbeta, red);
 }
 
-// blocks [0, nparam): dgamma / dbeta; the others: dx
+// Blocks [0, nparam): dgamma / dbeta; the others: dx = a dz - k1 - (x - mean) k2 from x and dy read again, dz formed again
+// (storing it would cost a write and a read of the map).  4 x 16384 x 512 bf16, SiLU: 41 us, 201 MB at 4.9 TB/s.
 template <typename T, int ACT, bool ONCE>
 __global__ __launch_bounds__(1024) void gn_bwd_apply_kernel(const T* __restrict__ dy, const T* __restrict__ x,
                                                             const float* __restrict__ gamma,
@@ -722,6 +731,9 @@ __global__ __launch_bounds__(1024) void gn_bwd_apply_kernel(const T* __restrict_
 //   m = sum x / N,  d = x - m,  mean = m + sum d / N,  var = (sum d^2 - (sum d)^2 / N) / N,
 // exact to rounding whatever the mean is.  A bundle has at least 64 bytes of a row where enough blocks remain; the
 // bundles of one sample run on one XCD, whose L2 they share.
+// One launch instead of three, one read instead of two.  256 x 512 x 128 bf16 in 16 groups, SiLU: 21 us, 67 MB at 3.2 TB/s
+// (chunks: 40 us); 32 x 2080 x 64 fp32 in 8 groups, ReLU: 15 us (22), backward 18.6 + 3.8 us (28); 1 x 2080 x 64: 5 us,
+// which is the launch and two joins.  Bound by the wait for a block's own loads: its two sums cannot start before.
 struct Slab {
   long S;          // values per sample
   int P, C, G, Cg;

@@ -387,6 +387,23 @@ def test_groups_of_many_and_of_two_channels(size, dtype):
 
 
 @pytest.mark.gpu
+def test_more_values_than_32_bits_count():
+    """33 samples of 2^26 values, 2.2 billion in all: the first and the last sample against the formula."""
+    from mmsa_amd.norm import group_norm_act
+    B, P, C, G = 33, 1 << 20, 64, 8
+    x = torch.randn(B, P, C, device=DEV, dtype=torch.bfloat16)
+    dy = torch.randn(B, P, C, device=DEV, dtype=torch.bfloat16)
+    w, b = torch.linspace(0.5, 1.5, C, device=DEV), torch.linspace(-1.0, 1.0, C, device=DEV)
+    leaf = x.transpose(1, 2).requires_grad_()
+    y = group_norm_act(leaf, G, w, b, 1e-5, "silu")
+    dx, = torch.autograd.grad(y, leaf, dy.transpose(1, 2))
+    for i in (0, B - 1):
+        want = formula(x[i:i + 1].detach().double(), w.double(), b.double(), G, 1e-5, "silu", dy[i:i + 1].double())
+        within(y[i:i + 1].detach().transpose(1, 2), *want[0], torch.bfloat16)
+        within(dx[i:i + 1].transpose(1, 2), *want[1], torch.bfloat16)
+
+
+@pytest.mark.gpu
 def test_a_batch_of_many_tiny_samples_and_one_of_few_long_ones():
     """The two ends of how a map is cut: 20 000 blocks of one row, and one sample that a whole launch shares."""
     from mmsa_amd.norm import group_norm_act
