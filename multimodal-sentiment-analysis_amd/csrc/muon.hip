@@ -694,40 +694,11 @@ __global__ __launch_bounds__(256, BT == 256 || Tile<BT>::LDS > 81920 ? 1 : 2) vo
   }
 }
 
-// Sums the partial tiles of the matrices whose K was split, four values (of one column) per lane: 4 to 8 us, nearly all of
-// it the launch and a chain of three dependent loads; 15 us for the 2048 x 8192 one.  Many parts are shared
-// out among a block's four waves; of few parts every wave adds up its own values.
-__host__ __device__ inline bool many_parts(int nsplit) { return nsplit >= 8; }
-
-template <int BT, int MODE>
-__global__ __launch_bounds__(256) void join_kernel(const Group* __restrict__ grp, int step) {
-  constexpr int W = Tile<BT>::W, PER = BT * BT / 256;          // groups of 64 x 4 values in a tile
-  __shared__ f32x4 sums[4][64];
-  const Group& gr = *grp;
-  const int mi = find_mat(gr.first[PH_JOIN + MODE], gr.count, blockIdx.x);
-  const Mat& q = gr.mat[mi];
-  const int b = blockIdx.x - gr.first[PH_JOIN + MODE][mi], lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int nsplit = q.nsplit[MODE];
-  const bool many = many_parts(nsplit);
-  const int unit = many ? b : b * 4 + wave, tile = unit / PER, r = unit % PER;
-  const int w = r & 3, g = (r >> 2) & 3, x = (r >> 4) / W, y = (r >> 4) % W;
-  const float* p = ws_part(q) + (long)tile * nsplit * (BT * BT) + ((x * W + y) * 16 + 4 * g) * 256 + w * 64 + lane;
-  f32x4 v = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 4
-  for (int s = many ? wave : 0; s < nsplit; s += many ? 4 : 1)
-#pragma unroll
-    for (int k = 0; k < 4; ++k) v[k] += p[(long)s * (BT * BT) + k * 256];
-  if (many) {
-    sums[wave][lane] = v;
-    __syncthreads();
-    if (wave) return;
-    v = (sums[0][lane] + sums[1][lane]) + (sums[2][lane] + sums[3][lane]);
-  }
-  int ti, tj;
-  lower_tile(tile, ti, tj);
+// Four values of T or B, rows i .. i + 3 of column j: scaled, as pairs, in their place and (outside the tiles of the
+// diagonal) its mirror image.
+template <int MODE>
+__device__ __forceinline__ void store_four(const Mat& q, int step, const f32x4& v, long i, long j, bool mirrored) {
   const float mul = result_scale<MODE>(q, step);
-  const long i = (long)ti * BT + (w >> 1) * W * 32 + x * 32 + 8 * g + 4 * (lane >> 5);
-  const long j = (long)tj * BT + (w & 1) * W * 32 + y * 32 + (lane & 31);
   char* dst = MODE == TO_T ? ws_t(q) : ws_b(q);
   f16x4 hi, lo;
 #pragma unroll
@@ -738,10 +709,126 @@ __global__ __launch_bounds__(256) void join_kernel(const Group* __restrict__ grp
     lo[k] = (_Float16)(o - (float)hi[k]);
     put_pair(dst, i + k, j, q.mp, o);
   }
-  if (ti == tj) return;
+  if (!mirrored) return;
   char* o = dst + j * row_bytes(q.mp) + (i >> 4) * 64 + (i & 15) * 2;
   *reinterpret_cast<f16x4*>(o) = hi;
   *reinterpret_cast<f16x4*>(o + 32) = lo;
+}
+
+// T or B in tiles of 32 x 32, for matrices whose larger tiles would leave most compute units without one: a step is 64
+// values of K, a quarter of it for each of the four waves, whose sums meet in LDS at the end.
+// 700 x 700, 253 tiles instead of 66: 135 us for the five steps instead of 163; the model's twelve convolutions need no
+// split of K for it, 140 us instead of 150.  Twice the bytes of a 64 tile per product: beyond a
+// block per compute unit it loses (1024 x 1024: 528 blocks).
+template <int MODE>
+__global__ __launch_bounds__(256, 2) void narrow_kernel(const Group* __restrict__ grp, int step) {
+  constexpr int RING = 4, ROW = 256, OPER = 32 * ROW, BUF = 2 * OPER, LOADS = 4;
+  __shared__ __attribute__((aligned(128))) char lds[RING * BUF];
+  const Group& gr = *grp;
+  const bool even = gr.even[MODE];
+  const int block = even ? xcd_order(blockIdx.x, gridDim.x) : blockIdx.x;
+  const int mi = find_mat(gr.first[PH_PRODUCT + MODE], gr.count, block);
+  const Mat& q = gr.mat[mi];
+  const int b = block - gr.first[PH_PRODUCT + MODE][mi];
+  const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int nt = q.mp / 32, nsplit = q.nsplit[MODE];
+  const int l = even ? b : xcd_order(b, nt * (nt + 1) / 2 * nsplit), tile = l / nsplit, part = l % nsplit;
+  int ti, tj;
+  lower_tile(tile, ti, tj);
+  const int K = MODE == TO_T ? q.np : q.mp, all = K / 64;
+  const int kper = (all + nsplit - 1) / nsplit, k_lo = part * kper, nk = all - k_lo < kper ? all - k_lo : kper;
+  const long pitch = row_bytes(K);
+  const char* X = (MODE == TO_T ? ws_x(q) : ws_t(q)) + (long)k_lo * ROW;
+  // a wave's load fills four rows; unit u of row r lies at u ^ (r & 15), so that 16 lanes of a fragment read cover all banks
+  const int row = 4 * w + (lane >> 4);
+  const char* ps = X + (ti * 32l + row) * pitch + ((lane & 15) ^ row) * 16;
+  const char* qs = X + (tj * 32l + row) * pitch + ((lane & 15) ^ row) * 16;
+  auto stage = [&](int k) {
+    char* to = lds + (k & (RING - 1)) * BUF + w * 1024;
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      load_lds16(ps + j * 16 * pitch + (long)k * ROW, to + j * 4096);
+      load_lds16(qs + j * 16 * pitch + (long)k * ROW, to + OPER + j * 4096);
+    }
+  };
+  const int fr = lane & 31, half = lane >> 5;
+  const int uh = fr * ROW + ((4 * w + half) ^ (fr & 15)) * 16, ul = fr * ROW + ((4 * w + 2 + half) ^ (fr & 15)) * 16;
+  f32x16 acc, low;
+#pragma unroll
+  for (int e = 0; e < 16; ++e) acc[e] = low[e] = 0.f;
+  for (int k = 0; k < RING - 1 && k < nk; ++k) stage(k);
+  for (int k = 0; k < nk; ++k) {
+    // the steps behind this one may still be on their way
+    if (k + 2 < nk)
+      wait_loads_and_meet<2 * LOADS>();
+    else if (k + 1 < nk)
+      wait_loads_and_meet<LOADS>();
+    else
+      wait_loads_and_meet<0>();
+    if (k + RING - 1 < nk) stage(k + RING - 1);       // into the buffer of step k - 1, which all waves have read
+    const char* l0 = lds + (k & (RING - 1)) * BUF;
+    const f16x8 ph = *reinterpret_cast<const f16x8*>(l0 + uh), pl = *reinterpret_cast<const f16x8*>(l0 + ul);
+    const f16x8 qh = *reinterpret_cast<const f16x8*>(l0 + OPER + uh), ql = *reinterpret_cast<const f16x8*>(l0 + OPER + ul);
+    low = __builtin_amdgcn_mfma_f32_32x32x16_f16(pl, qh, low, 0, 0, 0);
+    acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(ph, qh, acc, 0, 0, 0);
+    low = __builtin_amdgcn_mfma_f32_32x32x16_f16(ph, ql, low, 0, 0, 0);
+  }
+  __syncthreads();
+  float* sums = reinterpret_cast<float*>(lds);          // [wave][register][lane]
+#pragma unroll
+  for (int e = 0; e < 16; ++e) sums[(w * 16 + e) * 64 + lane] = acc[e] + low[e];
+  __syncthreads();
+  f32x4 v;
+#pragma unroll
+  for (int r = 0; r < 4; ++r) {
+    const float* p = sums + (4 * w + r) * 64 + lane;
+    v[r] = (p[0] + p[1024]) + (p[2048] + p[3 * 1024]);
+  }
+  if (nsplit > 1) {
+    float* o = ws_part(q) + ((long)tile * nsplit + part) * 1024 + 4 * w * 64 + lane;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) o[r * 64] = v[r];
+    return;
+  }
+  // register e of a lane: row (e & 3) + 8 (e >> 2) + 4 half, column fr
+  store_four<MODE>(q, step, v, ti * 32l + 8 * w + 4 * half, tj * 32l + fr, ti != tj);
+}
+
+// Sums the partial tiles of the matrices whose K was split, four values (of one column) per lane: 4 to 8 us, nearly all of
+// it the launch and a chain of three dependent loads; 15 us for the 2048 x 8192 one.  Many parts are shared
+// out among a block's four waves; of few parts every wave adds up its own values.
+__host__ __device__ inline bool many_parts(int nsplit) { return nsplit >= 8; }
+
+template <int BT, int MODE>
+__global__ __launch_bounds__(256) void join_kernel(const Group* __restrict__ grp, int step) {
+  constexpr int W = BT == 32 ? 1 : Tile<BT == 32 ? 64 : BT>::W, PER = BT * BT / 256;          // groups of 64 x 4 values in a tile
+  constexpr int WAVES = BT == 32 ? 1 : 4, REG = 64 * WAVES;    // waves that hold a tile, values of one register of them
+  __shared__ f32x4 sums[4][64];
+  const Group& gr = *grp;
+  const int mi = find_mat(gr.first[PH_JOIN + MODE], gr.count, blockIdx.x);
+  const Mat& q = gr.mat[mi];
+  const int b = blockIdx.x - gr.first[PH_JOIN + MODE][mi], lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int nsplit = q.nsplit[MODE];
+  const bool many = many_parts(nsplit);
+  const int unit = many ? b : b * 4 + wave, tile = unit / PER, r = unit % PER;
+  const int w = r % WAVES, g = r / WAVES & 3, x = r / (4 * WAVES) / W, y = r / (4 * WAVES) % W;
+  const float* p = ws_part(q) + (long)tile * nsplit * (BT * BT) + ((x * W + y) * 16 + 4 * g) * REG + w * 64 + lane;
+  f32x4 v = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+  for (int s = many ? wave : 0; s < nsplit; s += many ? 4 : 1)
+#pragma unroll
+    for (int k = 0; k < 4; ++k) v[k] += p[(long)s * (BT * BT) + k * REG];
+  if (many) {
+    sums[wave][lane] = v;
+    __syncthreads();
+    if (wave) return;
+    v = (sums[0][lane] + sums[1][lane]) + (sums[2][lane] + sums[3][lane]);
+  }
+  int ti, tj;
+  lower_tile(tile, ti, tj);
+  const long i = (long)ti * BT + (w >> 1) * W * 32 + x * 32 + 8 * g + 4 * (lane >> 5);
+  const long j = (long)tj * BT + (w & 1) * W * 32 + y * 32 + (lane & 31);
+  store_four<MODE>(q, step, v, i, j, ti != tj);
 }
 
 // ---- matrices that fit one block
@@ -1029,16 +1116,17 @@ long tri(long t) { return t * (t + 1) / 2; }
 
 // What a phase costs in microseconds with BT x BT tiles, from measurements (squares of 256 to 4096 values): a block
 // costs `start` plus `unit` per 32 values of K where it has a compute unit to itself and `full` where the chip is full
-// (64: two blocks share a unit).  Larger tiles read less per product, so they win once they fill the chip.
+// (32 and 64: two blocks share a unit).  Larger tiles read less per product, so they win once they fill the chip.
 struct TileCost {
   int bt, slots;
   float start, unit, full;
 };
-constexpr TileCost COST[3] = {{64, 512, 4.0f, 0.27f, 0.54f}, {128, 256, 7.4f, 0.49f, 0.77f}, {256, 256, 9.6f, 2.25f, 2.25f}};
+constexpr TileCost COST[4] = {
+    {32, 512, 4.2f, 0.13f, 0.32f}, {64, 512, 4.0f, 0.27f, 0.54f}, {128, 256, 7.4f, 0.49f, 0.77f}, {256, 256, 9.6f, 2.25f, 2.25f}};
 
 // blocks: how many, their K steps in all, the longest and the shortest of them
 float phase_cost(const TileCost& c, long blocks, long steps, long longest, long shortest) {
-  const float unit = blocks <= 256 ? c.unit + (c.full - c.unit) * (c.bt == 64 ? 0.f : blocks / 256.f) : c.full;
+  const float unit = blocks <= 256 ? c.unit + (c.full - c.unit) * (c.bt <= 64 ? 0.f : blocks / 256.f) : c.full;
   float rounds;
   if (longest == shortest)
     rounds = (float)((blocks + c.slots - 1) / c.slots);
@@ -1072,6 +1160,7 @@ void make_plan(const int* rows, const int* cols, Group* gr, Plan* pl) {
   float best = 0.f;
   int pad = 0;
   for (const TileCost& c : COST) {
+    if (c.bt == 32) continue;
     long blocks = 0, steps = 0, longest = 0, shortest = 1l << 40;
     for (int i = 0; i < n; ++i) {
       const long mt = mmsa_cdiv(d[i].m, c.bt), t = mt * mmsa_cdiv(d[i].n, c.bt), k = mt * c.bt / 32;
@@ -1194,6 +1283,12 @@ void launch_product(const Plan& pl, const Group* dev, int step, const Step& st, 
       return;
     }
   }
+  if constexpr (MODE < TO_X) {
+    if (pl.bt[PHASE] == 32) {
+      hipLaunchKernelGGL((narrow_kernel<MODE>), grid, dim3(256), 0, s, dev, step);
+      return;
+    }
+  }
   if (pl.bt[PHASE] == 128)
     hipLaunchKernelGGL((product_kernel<T, 128, MODE>), grid, dim3(256), 0, s, dev, step, step & 1, st.decay, st.rate);
   else
@@ -1205,6 +1300,8 @@ void launch_join(const Plan& pl, const Group* dev, int step, hipStream_t s) {
   if (!blocks) return;
   if (pl.bt[MODE] == 128)
     hipLaunchKernelGGL((join_kernel<128, MODE>), dim3(blocks), dim3(256), 0, s, dev, step);
+  else if (pl.bt[MODE] == 32)
+    hipLaunchKernelGGL((join_kernel<32, MODE>), dim3(blocks), dim3(256), 0, s, dev, step);
   else
     hipLaunchKernelGGL((join_kernel<64, MODE>), dim3(blocks), dim3(256), 0, s, dev, step);
 }

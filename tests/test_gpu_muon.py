@@ -90,6 +90,19 @@ def test_lists_of_small_matrices(longest):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("shapes", [[(65, 6000)], [(700, 700)], [(96, 20011)], [(130, 2600)], [(200, 30000)], [(385, 768)],
+                                    [(128, 1152)] * 30, [(200, 64), (70, 3000), (520, 520), (66, 66), (3, 4000)],
+                                    [(2600, 1300)]], ids=lambda v: "-".join("x".join(map(str, s)) for s in v[:5]))
+def test_tiles_and_splits(shapes):
+    """Sizes for which the symmetric products come in tiles of 32, 64 and 128, whole and with their K split, in one
+    launch with others."""
+    from mmsa_amd.muon import orthogonalize
+    gs = [grad(*s, seed=sum(s) + i) for i, s in enumerate(shapes)]
+    for s, g, o in zip(shapes, gs, orthogonalize(gs)):
+        close(o, ns64(g), tol(s))
+
+
+@pytest.mark.gpu
 def test_a_large_matrix():
     from mmsa_amd.muon import orthogonalize
     for shape in ((2048, 2100), (4097, 700)):
