@@ -436,11 +436,11 @@ MMSA_API int mmsa_copy_multi(const void* const* srcs, void* const* dsts, const l
  *      one GPU is too small for batch statistics; the formulas are torch.nn.GroupNorm's) ------------------------------
  * x, y, dy, dx: [batch][positions][channels] of `dtype` (MMSA_F32 / MMSA_BF16 / MMSA_F16); gamma, beta [channels] fp32,
  * each may be null (1 / 0); stats [batch][groups][2] doubles (mean, 1 / sqrt(var + eps)), written by the forward pass
- * and read by the backward pass.  act: MMSA_ACT_*.  dx, dgamma, dbeta may each be null (not wanted).  Results do not
+ * (null: not wanted) and read by the backward pass.  act: MMSA_ACT_*.  dx, dgamma, dbeta may each be null (not wanted).  Results do not
  * depend on the order in which workgroups run.  Limits (MMSA_ERR_LIMIT): 4096 channels; where the channels are no
  * multiple of a 16-byte vector, channels * (values per vector) / gcd at most 12288; 4 million samples, 16 million
  * groups or runs of 64 channels over all samples.
- * scratch: mmsa_group_norm_act_scratch_bytes(...) bytes, 8-byte aligned. */
+ * scratch: mmsa_group_norm_act_scratch_bytes(..., backward) bytes for either pass, 8-byte aligned, null where 0. */
 #define MMSA_F32 0
 #define MMSA_BF16 1
 #define MMSA_F16 2
@@ -448,7 +448,8 @@ MMSA_API int mmsa_copy_multi(const void* const* srcs, void* const* dsts, const l
 #define MMSA_ACT_RELU 1
 #define MMSA_ACT_SILU 2
 #define MMSA_ACT_GELU 3 /* erf form */
-MMSA_API long mmsa_group_norm_act_scratch_bytes(long batch, long positions, int channels, int groups, int dtype);
+MMSA_API long mmsa_group_norm_act_scratch_bytes(long batch, long positions, int channels, int groups, int dtype,
+                                                int backward);
 MMSA_API int mmsa_group_norm_act_fwd(const void* x, const float* gamma, const float* beta, void* y, double* stats,
                                      void* scratch, long batch, long positions, int channels, int groups, float eps,
                                      int act, int dtype, void* stream);

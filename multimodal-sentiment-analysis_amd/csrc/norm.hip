@@ -887,7 +887,7 @@ __global__ __launch_bounds__(1024) void gn_slab_fwd_kernel(const T* __restrict__
   const double mean64 = (double)m + off;
   // a NaN of the data passes fmax by: put it back
   const double rstd64 = sum[g][1] == sum[g][1] ? 1.0 / sqrt(var + (double)eps) : sum[g][1];
-  if (in && r0 == 0 && col * W % q.Cg == 0) {
+  if (stats && in && r0 == 0 && col * W % q.Cg == 0) {
     double* o = stats + 2 * (p.b * q.G + p.c0 / q.Cg + g);
     o[0] = mean64;
     o[1] = rstd64;
@@ -1239,6 +1239,8 @@ int gn_fwd(const void* x, const float* gamma, const float* beta, void* y, double
   const T* xp = static_cast<const T*>(x);
   T* yp = static_cast<T*>(y);
   double* part = static_cast<double*>(scratch);
+  MMSA_REQUIRE(scratch);
+  if (!stats) stats = part + batch * cut.nchunk * cut.G * 3;
   if (batch * cut.S * (long)sizeof(T) > GN_CACHED)
     return cut_fwd<T, true>(xp, gamma, beta, yp, stats, part, batch, cut, dtype, eps, act, s);
   return cut_fwd<T, false>(xp, gamma, beta, yp, stats, part, batch, cut, dtype, eps, act, s);
@@ -1315,20 +1317,23 @@ int check_size(long batch, long positions, int channels, int groups, int dtype, 
 
 }  // namespace
 
-// Bytes of scratch either direction needs for these sizes (the larger of the two; 8-byte aligned).
-MMSA_EXPORT long mmsa_group_norm_act_scratch_bytes(long batch, long positions, int channels, int groups, int dtype) {
+// Bytes of scratch the forward or the backward pass needs for these sizes (8-byte aligned; 0: none, it may be null).
+MMSA_EXPORT long mmsa_group_norm_act_scratch_bytes(long batch, long positions, int channels, int groups, int dtype,
+                                                   int backward) {
   Cut cut;
+  Slab q;
   if (int rc = check_size(batch, positions, channels, groups, dtype, &cut)) return rc;
-  const long fwd = batch * cut.nchunk * groups * 3 * 8;
-  const long bwd = (batch * cut.nchunk * channels + batch * channels + batch * groups) * 2 * 4;
-  return fwd > bwd ? fwd : bwd;
+  if (make_slab(batch, positions, channels, groups, dtype, backward ? BWD_REGS : FWD_REGS, backward, &q))
+    return backward ? batch * channels * 2 * 4 : 0;
+  if (backward) return (batch * cut.nchunk * channels + batch * channels + batch * groups) * 2 * 4;
+  return (batch * cut.nchunk * groups * 3 + batch * groups * 2) * 8;      // with a place for unwanted statistics
 }
 
-// y = act(group_norm(x) gamma + beta); stats [batch][groups][2] <- mean, 1 / sqrt(var + eps) in double
+// y = act(group_norm(x) gamma + beta); stats [batch][groups][2] <- mean, 1 / sqrt(var + eps) in double, null: not wanted
 MMSA_EXPORT int mmsa_group_norm_act_fwd(const void* x, const float* gamma, const float* beta, void* y, double* stats,
                                         void* scratch, long batch, long positions, int channels, int groups, float eps,
                                         int act, int dtype, void* stream) {
-  MMSA_REQUIRE(x && y && stats && scratch && act >= 0 && act <= 3 && eps >= 0.f);
+  MMSA_REQUIRE(x && y && act >= 0 && act <= 3 && eps >= 0.f);
   Cut cut;
   if (int rc = check_size(batch, positions, channels, groups, dtype, &cut)) return rc;
   hipStream_t s = mmsa_stream(stream);

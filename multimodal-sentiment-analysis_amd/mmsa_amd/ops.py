@@ -232,10 +232,12 @@ def _group_norm_check(C, groups, act, gamma, beta, device):
     if groups < 1 or C < 1 or C % groups:
         raise ValueError(f"group_norm_act: {C} channels do not divide into {groups} groups")
     for t, name in ((gamma, "weight"), (beta, "bias")):
-        if t is not None and tuple(t.shape) != (C,):
+        if t is None:
+            continue
+        if t.shape != (C,):
             raise ValueError(f"group_norm_act: {name} must be [{C}]")
-        if t is not None and t.device != device:
-            raise _lib.MmsaError(f"group_norm_act: {name} lives on {t.device}, the map on {device}")
+        if t.get_device() != device:
+            raise _lib.MmsaError(f"group_norm_act: {name} lives on {t.device}, the map on GPU {device}")
 
 
 def _group_norm_args(x, gamma, beta, groups, act):
@@ -243,27 +245,30 @@ def _group_norm_args(x, gamma, beta, groups, act):
         raise ValueError("group_norm_act: x must be [B, positions, channels]")
     if x.dtype not in DTYPE_CODES:
         raise TypeError(f"group_norm_act: float32, bfloat16 or float16 maps, got {x.dtype}")
-    _group_norm_check(x.shape[2], groups, act, gamma, beta, x.device)
+    _group_norm_check(x.shape[2], groups, act, gamma, beta, x.get_device())
     return x.shape
 
 
-@functools.lru_cache(maxsize=256)
-def _group_norm_scratch_doubles(B, P, C, groups, code):
-    return (_lib.query("mmsa_group_norm_act_scratch_bytes", B, P, C, groups, code) + 7) // 8
+@functools.lru_cache(maxsize=512)
+def _group_norm_scratch_doubles(B, P, C, groups, code, backward):
+    return (_lib.query("mmsa_group_norm_act_scratch_bytes", B, P, C, groups, code, backward) + 7) // 8
 
 
 def _group_norm_launch_fwd(x, gamma, beta, y, stats, B, P, C, groups, eps, act):
-    """The launch alone, for a caller that has checked layouts itself: x and y hold [B, P, C] one value after another."""
+    """The launch alone, for a caller that has checked layouts itself: x and y hold [B, P, C] one value after another;
+    stats may be None."""
     code = DTYPE_CODES[x.dtype]
-    scratch = torch.empty(_group_norm_scratch_doubles(B, P, C, groups, code), dtype=torch.float64, device=x.device)
+    need = _group_norm_scratch_doubles(B, P, C, groups, code, 0)
+    scratch = torch.empty(need, dtype=torch.float64, device=x.device) if need else None
     _OPERANDS.dev = x.get_device()
     _lib.call("mmsa_group_norm_act_fwd", x.data_ptr(), _opt(gamma, F32, "weight"), _opt(beta, F32, "bias"), y.data_ptr(),
-              stats.data_ptr(), scratch.data_ptr(), B, P, C, groups, eps, ACTIVATIONS[act], code, _stream())
+              None if stats is None else stats.data_ptr(), None if scratch is None else scratch.data_ptr(), B, P, C,
+              groups, eps, ACTIVATIONS[act], code, _stream())
 
 
 def _group_norm_launch_bwd(dy, x, gamma, beta, stats, dx, dgamma, dbeta, B, P, C, groups, act):
     code = DTYPE_CODES[x.dtype]
-    scratch = torch.empty(_group_norm_scratch_doubles(B, P, C, groups, code), dtype=torch.float64, device=x.device)
+    scratch = torch.empty(_group_norm_scratch_doubles(B, P, C, groups, code, 1), dtype=torch.float64, device=x.device)
     _OPERANDS.dev = x.get_device()
     _lib.call("mmsa_group_norm_act_bwd", dy.data_ptr(), x.data_ptr(), None if gamma is None else gamma.data_ptr(),
               None if beta is None else beta.data_ptr(), stats.data_ptr(), None if dx is None else dx.data_ptr(),

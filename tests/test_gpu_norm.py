@@ -451,9 +451,12 @@ def test_refusals():
         ops.group_norm_act_bwd(x, x, None, None, st, x[:1], None, None, 2)
     one = 1 << 12
     q = lib.mmsa_group_norm_act_scratch_bytes
-    assert q(1, 1, 8, 3, 0) == -1 and q(0, 1, 8, 2, 0) == -1 and q(1, 1, 8, 2, 3) == -1
-    assert q(1, 1, 4097, 1, 0) == -3 and q(5_000_000, 1, 8, 1, 0) == -3 and q(1, 1, 1537, 1, 1) == -3
-    assert q(2, 100, 64, 8, 1) > 0
+    for backward in (0, 1):
+        assert q(1, 1, 8, 3, 0, backward) == -1 and q(0, 1, 8, 2, 0, backward) == -1 and q(1, 1, 8, 2, 3, backward) == -1
+        assert q(1, 1, 4097, 1, 0, backward) == -3 and q(5_000_000, 1, 8, 1, 0, backward) == -3
+        assert q(1, 1, 1537, 1, 1, backward) == -3 and q(2, 100000, 64, 8, 1, backward) > 0
+    assert q(2, 100, 64, 8, 1, 0) == 0 and q(2, 100, 64, 8, 1, 1) == 2 * 64 * 8      # a sample's groups fit a block each
+    assert lib.mmsa_group_norm_act_fwd(one, None, None, one, None, None, 2, 100000, 64, 8, 1e-5, 0, 1, None) == -1
     assert lib.mmsa_group_norm_act_fwd(None, None, None, one, one, one, 1, 1, 8, 2, 1e-5, 0, 0, None) == -1
     assert lib.mmsa_group_norm_act_fwd(one, None, None, one, one, one, 1, 1, 8, 3, 1e-5, 0, 0, None) == -1
     assert lib.mmsa_group_norm_act_fwd(one, None, None, one, one, one, 1, 1, 8, 2, 1e-5, 4, 0, None) == -1
