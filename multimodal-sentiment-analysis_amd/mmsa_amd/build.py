@@ -36,14 +36,15 @@ def _stale(target: str, deps) -> bool:
 def build(force: bool = False, verbose: bool = False) -> str:
     os.makedirs(OBJ_DIR, exist_ok=True)
     hipcc = _hipcc()
-    headers = tuple(os.path.join(CSRC, h) for h in ("mmsa_common.h", "fft512.h", "conv_rows3.h"))
+    # what every object depends on; this file for its flags
+    shared = (*(os.path.join(CSRC, h) for h in ("mmsa_common.h", "fft512.h", "conv_rows3.h")), os.path.abspath(__file__))
     jobs = []
     objs = []
     for src in SOURCES:
         s = os.path.join(CSRC, src)
         o = os.path.join(OBJ_DIR, src.replace(".hip", ".o"))
         objs.append(o)
-        if force or _stale(o, (s, *headers)):
+        if force or _stale(o, (s, *shared)):
             jobs.append([hipcc, *FLAGS, "-c", s, "-o", o])
 
     def run(cmd):
