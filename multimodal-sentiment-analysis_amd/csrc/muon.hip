@@ -77,10 +77,13 @@ __device__ __forceinline__ char* ws_b(const Mat& q) { return q.ws + xbytes(q) + 
 __device__ __forceinline__ int* ws_k(const Mat& q) { return reinterpret_cast<int*>(q.ws + mat_bytes(q) - 128); }
 __device__ __forceinline__ float* ws_part(const Mat& q) { return reinterpret_cast<float*>(q.ws + mat_bytes(q)); }
 
-// which matrix a block works on: the last one whose first block is not behind it (all lanes of a wave call it)
+// Which matrix a block works on: the last one whose first block is not behind it (all lanes of a wave call it).  `count`
+// is a kernel argument, as is all that a block needs before it can ask for its descriptor: every load that waits for
+// another one here is a microsecond of every launch.
 __device__ __forceinline__ int find_mat(const int* first, int count, int block) {
+  if (count == 1) return 0;
   const int lane = threadIdx.x & 63;
-  const bool at_or_behind = lane < count && first[lane < count ? lane : 0] <= block;
+  const bool at_or_behind = first[lane < GROUP ? lane : 0] <= block && lane < count;
   // matrices without a block in this launch share their first block with the next one that has some
   return __builtin_amdgcn_readfirstlane(__popcll(__ballot(at_or_behind)) - 1);
 }
@@ -208,12 +211,12 @@ __device__ __forceinline__ int extra_scale(double r) {
 // lanes write 256 consecutive bytes of a row.  Bound by memory: 33.6 M values with momentum 101 us, 537 MB at 5.3 TB/s.
 // Every block adds up the (at most 512) partial sums of its matrix itself, which spares a launch.
 template <typename T, bool MOM>
-__global__ __launch_bounds__(256) void split_kernel(const Group* __restrict__ grp, float mu, int nesterov, float eps,
+__global__ __launch_bounds__(256) void split_kernel(const Group* __restrict__ grp, int count, float mu, int nesterov, float eps,
                                                     int steps, const double* __restrict__ parts) {
   __shared__ double red[16];
   __shared__ float tile[64][65];
   const Group& gr = *grp;
-  const int i = find_mat(gr.first[PH_SPLIT], gr.count, blockIdx.x);
+  const int i = find_mat(gr.first[PH_SPLIT], count, blockIdx.x);
   const Mat& q = gr.mat[i];
   const int b = blockIdx.x - gr.first[PH_SPLIT][i];
   const bool tall = q.rows > q.cols;
@@ -500,16 +503,15 @@ __device__ __forceinline__ void multiply(f32x16 (&acc)[Tile<BT>::W][Tile<BT>::W]
 // image.  Where a phase has few tiles and a long K, a share of the K steps goes to one block each and the partial
 // results meet in join_kernel.
 template <typename T, int BT, int MODE>
-__global__ __launch_bounds__(256, BT == 256 || Tile<BT>::LDS > 81920 ? 1 : 2) void product_kernel(const Group* __restrict__ grp, int step,
-                                                                         int which, float decay, float rate) {
+__global__ __launch_bounds__(256, BT == 256 || Tile<BT>::LDS > 81920 ? 1 : 2) void product_kernel(
+    const Group* __restrict__ grp, int count, int even, int step, int which, float decay, float rate) {
   typedef Tile<BT> S;
   constexpr int W = S::W;
   __shared__ __attribute__((aligned(128))) char lds[S::LDS];
   const Group& gr = *grp;
   constexpr int PHASE = MODE < TO_X ? MODE : TO_X;
-  const bool even = gr.even[PHASE];
   const int block = even ? xcd_order(blockIdx.x, gridDim.x) : blockIdx.x;
-  const int mi = find_mat(gr.first[PH_PRODUCT + PHASE], gr.count, block);
+  const int mi = find_mat(gr.first[PH_PRODUCT + PHASE], count, block);
   const Mat& q = gr.mat[mi];
   const int b = block - gr.first[PH_PRODUCT + PHASE][mi];
   const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
@@ -721,13 +723,13 @@ __device__ __forceinline__ void store_four(const Mat& q, int step, const f32x4& 
 // split of K for it, 140 us instead of 150.  Twice the bytes of a 64 tile per product: beyond a
 // block per compute unit it loses (1024 x 1024: 528 blocks).
 template <int MODE>
-__global__ __launch_bounds__(256, 2) void narrow_kernel(const Group* __restrict__ grp, int step) {
+__global__ __launch_bounds__(256, 2) void narrow_kernel(const Group* __restrict__ grp, int count, int even,
+                                                            int step) {
   constexpr int RING = 4, ROW = 256, OPER = 32 * ROW, BUF = 2 * OPER, LOADS = 4;
   __shared__ __attribute__((aligned(128))) char lds[RING * BUF];
   const Group& gr = *grp;
-  const bool even = gr.even[MODE];
   const int block = even ? xcd_order(blockIdx.x, gridDim.x) : blockIdx.x;
-  const int mi = find_mat(gr.first[PH_PRODUCT + MODE], gr.count, block);
+  const int mi = find_mat(gr.first[PH_PRODUCT + MODE], count, block);
   const Mat& q = gr.mat[mi];
   const int b = block - gr.first[PH_PRODUCT + MODE][mi];
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -800,12 +802,12 @@ __global__ __launch_bounds__(256, 2) void narrow_kernel(const Group* __restrict_
 __host__ __device__ inline bool many_parts(int nsplit) { return nsplit >= 8; }
 
 template <int BT, int MODE>
-__global__ __launch_bounds__(256) void join_kernel(const Group* __restrict__ grp, int step) {
+__global__ __launch_bounds__(256) void join_kernel(const Group* __restrict__ grp, int count, int step) {
   constexpr int W = BT == 32 ? 1 : Tile<BT == 32 ? 64 : BT>::W, PER = BT * BT / 256;          // groups of 64 x 4 values in a tile
   constexpr int WAVES = BT == 32 ? 1 : 4, REG = 64 * WAVES;    // waves that hold a tile, values of one register of them
   __shared__ f32x4 sums[4][64];
   const Group& gr = *grp;
-  const int mi = find_mat(gr.first[PH_JOIN + MODE], gr.count, blockIdx.x);
+  const int mi = find_mat(gr.first[PH_JOIN + MODE], count, blockIdx.x);
   const Mat& q = gr.mat[mi];
   const int b = blockIdx.x - gr.first[PH_JOIN + MODE][mi], lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int nsplit = q.nsplit[MODE];
@@ -1274,36 +1276,39 @@ struct Step {
 };
 
 template <typename T, int MODE>
-void launch_product(const Plan& pl, const Group* dev, int step, const Step& st, hipStream_t s) {
+void launch_product(const Plan& pl, const Group& gr, const Group* dev, int step, const Step& st, hipStream_t s) {
   constexpr int PHASE = MODE < TO_X ? MODE : TO_X;
   const dim3 grid(pl.blocks[PH_PRODUCT + PHASE]);
   if constexpr (MODE >= TO_X) {
     if (pl.bt[PHASE] == 256) {
-      hipLaunchKernelGGL((product_kernel<T, 256, MODE>), grid, dim3(256), 0, s, dev, step, step & 1, st.decay, st.rate);
+      hipLaunchKernelGGL((product_kernel<T, 256, MODE>), grid, dim3(256), 0, s, dev, gr.count, gr.even[PHASE], step,
+                       step & 1, st.decay, st.rate);
       return;
     }
   }
   if constexpr (MODE < TO_X) {
     if (pl.bt[PHASE] == 32) {
-      hipLaunchKernelGGL((narrow_kernel<MODE>), grid, dim3(256), 0, s, dev, step);
+      hipLaunchKernelGGL((narrow_kernel<MODE>), grid, dim3(256), 0, s, dev, gr.count, gr.even[PHASE], step);
       return;
     }
   }
   if (pl.bt[PHASE] == 128)
-    hipLaunchKernelGGL((product_kernel<T, 128, MODE>), grid, dim3(256), 0, s, dev, step, step & 1, st.decay, st.rate);
+    hipLaunchKernelGGL((product_kernel<T, 128, MODE>), grid, dim3(256), 0, s, dev, gr.count, gr.even[PHASE], step,
+                       step & 1, st.decay, st.rate);
   else
-    hipLaunchKernelGGL((product_kernel<T, 64, MODE>), grid, dim3(256), 0, s, dev, step, step & 1, st.decay, st.rate);
+    hipLaunchKernelGGL((product_kernel<T, 64, MODE>), grid, dim3(256), 0, s, dev, gr.count, gr.even[PHASE], step,
+                       step & 1, st.decay, st.rate);
 }
 template <int MODE>
-void launch_join(const Plan& pl, const Group* dev, int step, hipStream_t s) {
+void launch_join(const Plan& pl, const Group& gr, const Group* dev, int step, hipStream_t s) {
   const int blocks = pl.blocks[PH_JOIN + MODE];
   if (!blocks) return;
   if (pl.bt[MODE] == 128)
-    hipLaunchKernelGGL((join_kernel<128, MODE>), dim3(blocks), dim3(256), 0, s, dev, step);
+    hipLaunchKernelGGL((join_kernel<128, MODE>), dim3(blocks), dim3(256), 0, s, dev, gr.count, step);
   else if (pl.bt[MODE] == 32)
-    hipLaunchKernelGGL((join_kernel<32, MODE>), dim3(blocks), dim3(256), 0, s, dev, step);
+    hipLaunchKernelGGL((join_kernel<32, MODE>), dim3(blocks), dim3(256), 0, s, dev, gr.count, step);
   else
-    hipLaunchKernelGGL((join_kernel<64, MODE>), dim3(blocks), dim3(256), 0, s, dev, step);
+    hipLaunchKernelGGL((join_kernel<64, MODE>), dim3(blocks), dim3(256), 0, s, dev, gr.count, step);
 }
 
 // raising a kernel's LDS limit belongs to the device that is current
@@ -1373,17 +1378,17 @@ int run_all(const void* const* src, void* const* dst, void* const* mom, const in
     double* parts = reinterpret_cast<double*>(static_cast<char*>(scratch) + (sizeof(Group) + 127) / 128 * 128);
     hipLaunchKernelGGL((momentum_sumsq_kernel<T, MOM>), dim3(pl.blocks[PH_SUMSQ]), dim3(256), 0, s, gr, st.mu,
                        st.one_minus_mu, st.nesterov, parts, dev);
-    hipLaunchKernelGGL((split_kernel<T, MOM>), dim3(pl.blocks[PH_SPLIT]), dim3(256), 0, s, dev, st.mu, st.nesterov,
+    hipLaunchKernelGGL((split_kernel<T, MOM>), dim3(pl.blocks[PH_SPLIT]), dim3(256), 0, s, dev, gr.count, st.mu, st.nesterov,
                        st.eps, st.steps, parts);
     for (int t = 0; t < st.steps; ++t) {
-      launch_product<float, TO_T>(pl, dev, t, st, s);
-      launch_join<TO_T>(pl, dev, t, s);
-      launch_product<float, TO_B>(pl, dev, t, st, s);
-      launch_join<TO_B>(pl, dev, t, s);
+      launch_product<float, TO_T>(pl, gr, dev, t, st, s);
+      launch_join<TO_T>(pl, gr, dev, t, s);
+      launch_product<float, TO_B>(pl, gr, dev, t, st, s);
+      launch_join<TO_B>(pl, gr, dev, t, s);
       if (t + 1 < st.steps)
-        launch_product<float, TO_X>(pl, dev, t, st, s);
+        launch_product<float, TO_X>(pl, gr, dev, t, st, s);
       else
-        launch_product<T, MOM ? TO_PARAM : TO_OUT>(pl, dev, t, st, s);
+        launch_product<T, MOM ? TO_PARAM : TO_OUT>(pl, gr, dev, t, st, s);
     }
     if (int rc = mmsa_launch_status()) return rc;
   }
