@@ -11,6 +11,7 @@ import math
 
 import torch
 import torch.nn as nn
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _lib, ops
@@ -69,7 +70,8 @@ def group_norm_act(x: torch.Tensor, num_groups: int, weight=None, bias=None, eps
     float32, bfloat16 or float16 maps; ``weight`` / ``bias`` [C] float32 or None; activation "none", "relu", "silu" or
     "gelu" (erf form).  Maps in channels-last memory (what the convolutions here return) are used as they lie, others
     are copied into that order; the result is in channels-last memory.  Statistics and parameter gradients are held in
-    32 bits or more whatever the map's type.  Gradients flow to x, weight and bias (once: no gradient of a gradient).
+    32 bits or more whatever the map's type.  Gradients flow to x, weight and bias (once: no gradient of a gradient; no
+    forward-mode derivatives).
     """
     if x.dim() < 2:
         raise ValueError("group_norm_act: x must be [B, C, *positions]")
@@ -83,6 +85,9 @@ def group_norm_act(x: torch.Tensor, num_groups: int, weight=None, bias=None, eps
     if torch.is_grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad)
                                     or (bias is not None and bias.requires_grad)):
         return _GroupNormActFn.apply(x, weight, bias, num_groups, eps, activation)
+    # a dual tensor asks for no gradient; past the node, which refuses it, its tangent would get lost without a word
+    if any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in (x, weight, bias)):
+        raise NotImplementedError("group_norm_act has no forward-mode derivative (jvp)")
     y = torch.empty_like(x)
     if y.numel():
         ops._group_norm_launch_fwd(x, weight, bias, y, None, B, math.prod(x.shape[2:]), C, num_groups, eps, activation)
