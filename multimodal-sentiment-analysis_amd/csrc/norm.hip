@@ -127,6 +127,11 @@ struct Cut {
   int team;        // lanes that join the statistics of a group, a power of two up to a wave
 };
 
+// A thread's chain of 32-bit additions is a run of at most this many rows; the totals of a chunk's runs, at most as many,
+// are a second chain.  One chain for a whole chunk would drift as maps grow: equal addends by 170 half units over 1024
+// rows, by 10 over 64.
+constexpr int GN_RUN = 64;
+
 // sum over aligned teams of `team` lanes, the same in every lane of a team
 __device__ __forceinline__ double team_sum(double v, int team) {
   for (int s = 1; s < team; s <<= 1) v += __shfl_xor(v, s);
@@ -447,9 +452,10 @@ struct Channel {
   }
 };
 
-// Per chunk and channel: sum of dz and of dz xhat (rstd is one factor, applied at the end).  A thread sums 32 to 64 rows
-// in 32 bits, the block joins its threads, the chunks are joined in 64 bits.  4 x 16384 x 512 bf16, SiLU: 31 us, 134 MB at
-// 4.3 TB/s; the vector unit is as busy as memory (the slope of an activation is 12 to 20 instructions a value).
+// Per chunk and channel: sum of dz and of dz xhat (rstd is one factor, applied at the end).  A thread sums runs of at most
+// 64 rows in 32 bits and adds them up in its place in LDS; threads and chunks are joined in 64 bits, their sums kept in
+// 32 in between.  4 x 16384 x 512 bf16, SiLU: 31 us, 134 MB at 4.3 TB/s; the vector unit is as busy as memory (the slope
+// of an activation is 12 to 20 instructions a value).
 template <typename T, int ACT, bool ONCE>
 __global__ __launch_bounds__(1024) void gn_bwd_sums_kernel(const T* __restrict__ dy, const T* __restrict__ x,
                                                            const float* __restrict__ gamma,
@@ -472,15 +478,25 @@ __global__ __launch_bounds__(1024) void gn_bwd_sums_kernel(const T* __restrict__
     k.load(stats + 2 * b * cut.G, gamma, beta, (int)(((long)t * V) % cut.C), cut.C, cut.Cg);
     float s1[V], s2[V];           // sums of dz and of dz (x - mean)
 #pragma unroll
-    for (int e = 0; e < V; ++e) s1[e] = s2[e] = 0.f;
+    for (int e = 0; e < V; ++e) sh[t * V + e] = sh[slots + t * V + e] = s1[e] = s2[e] = 0.f;
     auto add = [&](int e, float v, float h) {
       float d;
       const float dz = k.template grad<ACT>(e, v, h, d);
       s1[e] += dz;
       s2[e] = fmaf(dz, d, s2[e]);
     };
+    // a run's sums are added to those before it in the thread's place in LDS
+    auto leave = [&]() {
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        sh[t * V + e] += s1[e];
+        sh[slots + t * V + e] += s2[e];
+        s1[e] = s2[e] = 0.f;
+      }
+    };
     int it = 0;
     for (; it + U <= me.full; it += U, p += U * hop, g += U * hop) {
+      if (it && it % GN_RUN == 0) leave();
       Pack<T, V> f[U], h[U];
 #pragma unroll
       for (int u = 0; u < U; ++u) {
@@ -509,22 +525,20 @@ __global__ __launch_bounds__(1024) void gn_bwd_sums_kernel(const T* __restrict__
       for (int e = 0; e < V; ++e) add(e, v[e], d[e]);
     }
 #pragma unroll
-    for (int e = 0; e < V; ++e) {
+    for (int e = 0; e < V; ++e)
       if (e < me.rest) add(e, Io<T>::to(p[e]), Io<T>::to(g[e]));
-      sh[t * V + e] = s1[e];
-      sh[slots + t * V + e] = s2[e];
-    }
+    leave();
   }
   __syncthreads();
   for (int c = tid; c < cut.C; c += blockDim.x) {
-    float a = 0.f, q = 0.f;
+    double a = 0.0, q = 0.0;
     for (int r = c; r < slots; r += cut.C) {
-      a += sh[r];
-      q += sh[slots + r];
+      a += (double)sh[r];
+      q += (double)sh[slots + r];
     }
     float* o = part + ((long)blockIdx.x * cut.C + c) * 2;
-    o[0] = a;
-    o[1] = q * (float)stats[2 * (b * cut.G + c / cut.Cg) + 1];
+    o[0] = (float)a;
+    o[1] = (float)(q * stats[2 * (b * cut.G + c / cut.Cg) + 1]);
   }
 }
 
@@ -1079,6 +1093,7 @@ bool make_cut(long batch, long positions, int C, int G, int dtype, Cut* cut) {
   // floats a channel, written and read again
   const long deep = 32l * C / ((long)V * cut->row);
   if (iters < deep) iters = deep < rows * batch / 256 ? deep : iters > rows * batch / 256 ? iters : rows * batch / 256;
+  if (iters > GN_RUN * GN_RUN) iters = GN_RUN * GN_RUN;
   if (iters > rows) iters = rows;
   cut->iters = (int)iters;
   cut->nchunk = (rows + iters - 1) / iters;

@@ -9,6 +9,30 @@ DEV = "cuda"
 U = 2.0 ** -24
 
 
+LONG = (1, 2 ** 24, 64, 8)          # one sample of 2^30 float32 values: a thread walks about a thousand rows of its block
+
+
+@pytest.mark.gpu
+def test_parameter_gradients_of_a_long_map():
+    """Sums of equal addends, the case in which a long chain of 32-bit additions drifts: runs of 64 rows (64 u at most),
+    sixteen runs a thread (16 u), the rest in 64 bits with a rounding of each chunk's and the final sum; rstd's own 2 u."""
+    import mmsa_amd.torch_ops  # noqa: F401
+    B, P, C, G = LONG
+    sign = torch.ones(P, device=DEV)
+    sign.view(-1, 2, P // 1024)[:, 1] = -1                # whole rows of one sign: mean 0, variance 1, both exact
+    x = sign.view(1, P, 1).expand(B, P, C).contiguous()
+    y, stats = torch.empty_like(x), torch.empty(B, G, 2, dtype=torch.float64, device=DEV)
+    torch.ops.mmsa.group_norm_act_fwd(x, None, None, y, stats, G, 1e-5, "none")
+    dw, db = torch.empty(C, device=DEV), torch.empty(C, device=DEV)
+    dy = torch.full_like(y, 0.7)
+    c = dy[0, 0, 0].double().item()
+    torch.ops.mmsa.group_norm_act_bwd(dy, x, None, None, stats, None, dw, db, G, "none")
+    assert float((db.double() / (c * P) - 1).abs().max()) <= 84 * U
+    torch.mul(x, 0.7, out=dy)
+    torch.ops.mmsa.group_norm_act_bwd(dy, x, None, None, stats, None, dw, db, G, "none")
+    assert float((dw.double() / (c * P / math.sqrt(1 + 1e-5)) - 1).abs().max()) <= 88 * U
+
+
 @pytest.mark.gpu
 def test_forward_mode_tangents_are_refused():
     """A dual tensor needs no gradient of its own, so it has to be looked for: its tangent must not get lost."""
