@@ -13,6 +13,24 @@ LONG = (1, 2 ** 24, 64, 8)          # one sample of 2^30 float32 values: a threa
 
 
 @pytest.mark.gpu
+def test_statistics_of_a_long_map_whose_first_rows_stand_apart():
+    """The first rows, from which every thread takes its origin, are 0 and all others 0.7.  In a run of 64 rows about
+    that origin the sum of squares 63 c^2 rounds to 64 u of itself at most, against a thread's whole sum of squares about
+    its mean of c^2: 64 * 64 u of the variance.  Later runs have an origin among their own values; sixteen of them are
+    joined in 32 bits, then all threads in 64.  The mean: a run's sum 64 u, sixteen joins, its own rounding."""
+    import mmsa_amd.torch_ops  # noqa: F401
+    B, P, C, G = LONG
+    x = torch.full((B, P, C), 0.7, device=DEV)
+    x[:, :P // 1024] = 0
+    y, stats = torch.empty_like(x), torch.empty(B, G, 2, dtype=torch.float64, device=DEV)
+    torch.ops.mmsa.group_norm_act_fwd(x, None, None, y, stats, G, 0.0, "none")
+    c, share = x[0, -1, 0].double().item(), 1 / 1024
+    assert float((stats[..., 0] / (c * (1 - share)) - 1).abs().max()) <= 84 * U
+    var = stats[..., 1] ** -2
+    assert float((var / (c * c * share * (1 - share)) - 1).abs().max()) <= 64 * 68 * U
+
+
+@pytest.mark.gpu
 def test_parameter_gradients_of_a_long_map():
     """Sums of equal addends, the case in which a long chain of 32-bit additions drifts: runs of 64 rows (64 u at most),
     sixteen runs a thread (16 u), the rest in 64 bits with a rounding of each chunk's and the final sum; rstd's own 2 u."""
