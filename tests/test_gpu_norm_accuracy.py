@@ -9,6 +9,54 @@ DEV = "cuda"
 U = 2.0 ** -24
 
 
+def pointwise64(z, act):
+    """The activation and its slope in 64 bits, each with the bound of a good 32-bit evaluation's error at 32-bit z and
+    of a 16-bit map's.
+
+    Phi(z) is erfc(-z / sqrt 2) / 2: its argument carries two roundings, which z < 0 magnifies by z^2 + 1, erfc itself
+    4 u.  exp(-z^2 / 2) rounds its argument (z^2 / 2 of it) and itself.  sigmoid: exp 2 u, sum u, quotient u.  For 16-bit
+    maps the normal tail is a polynomial good to 4e-6 of it, and exponentials take their argument times log2 e (three
+    roundings of it)."""
+    z = z.double()
+    if act == "silu":
+        s = torch.sigmoid(z)
+        y, slope = z * s, s * (1 + z * (1 - s))
+        r32, r16 = 8 * U * torch.ones_like(z), (2 * z.abs() + 10) * U
+        return y, slope, [(r * y.abs(), r * (slope.abs() + s * (1 + z.abs()))) for r in (r32, r16)]
+    phi = 0.5 * torch.special.erfc(-z / math.sqrt(2))
+    hill = z * torch.exp(-0.5 * z * z) / math.sqrt(2 * math.pi)
+    y, slope = z * phi, phi + hill
+    r32, r16 = (2 * z * z + 10) * U, 4e-6 + (1.5 * z * z + 12) * U
+    return y, slope, [(r * y.abs(), r * (phi + hill.abs())) for r in (r32, r16)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("positions", [2, 3000])                       # in registers, and cut into chunks
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16], ids=str)
+@pytest.mark.parametrize("act", ["silu", "gelu"])
+def test_activations_keep_their_digits_in_the_tails(act, dtype, positions):
+    """A weight of zero puts every channel's value at its bias, so that the activation and (as the bias gradient of one
+    unit in one place) its slope can be read off: relative accuracy from -12 to 12."""
+    from mmsa_amd.norm import group_norm_act
+    C = 1024
+    z = torch.linspace(-12, 12, C, device=DEV)
+    x = torch.randn(1, positions, C, device=DEV, generator=torch.Generator(device=DEV).manual_seed(1)).to(dtype)
+    bias = z.clone().requires_grad_()
+    y = group_norm_act(x.transpose(1, 2), 1, torch.zeros(C, device=DEV), bias, 1e-5, act)
+    dy = torch.zeros_like(y)
+    dy[0, :, 0] = 1
+    slope, = torch.autograd.grad(y, bias, dy)
+    want, want_slope, bounds = pointwise64(z, act)
+    ey, es = bounds[0 if dtype == torch.float32 else 1]
+    half = 0.0 if dtype == torch.float32 else torch.finfo(dtype).eps / 2
+    tiny = torch.finfo(dtype).tiny * torch.finfo(dtype).eps / 2
+    off = (y.detach().double() - want.view(1, C, 1)).abs()
+    assert bool((off <= (ey + half * want.abs() + tiny).view(1, C, 1)).all()), \
+        float((off / (ey + half * want.abs() + tiny).view(1, C, 1)).max())
+    off = (slope.double() - want_slope).abs()
+    assert bool((off <= es).all()), float((off / es).max())
+
+
 LONG = (1, 2 ** 24, 64, 8)          # one sample of 2^30 float32 values: a thread walks about a thousand rows of its block
 
 
