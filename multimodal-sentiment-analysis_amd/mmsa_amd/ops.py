@@ -231,6 +231,8 @@ def _group_norm_check(C, groups, act, gamma, beta, device):
         raise ValueError(f"group_norm_act: activation {act!r} is none of {', '.join(ACTIVATIONS)}")
     if groups < 1 or C < 1 or C % groups:
         raise ValueError(f"group_norm_act: {C} channels do not divide into {groups} groups")
+    if C >= 2 ** 31:            # the library takes an int, which would hold the count's low 32 bits
+        raise _lib.MmsaError(f"group_norm_act: limit exceeded: {C} channels")
     for t, name in ((gamma, "weight"), (beta, "bias")):
         if t is None:
             continue

@@ -119,3 +119,10 @@ def test_forward_mode_tangents_are_refused():
     with torch.autograd.forward_ad.dual_level():
         y = m(x)
     assert y.requires_grad
+
+
+def test_channel_counts_that_32_bits_cannot_hold_are_refused():
+    from mmsa_amd import _lib, ops
+    for C in (2 ** 31, 2 ** 32 + 8):
+        with pytest.raises(_lib.MmsaError, match="limit"):
+            ops._group_norm_check(C, 1, "none", None, None, 0)
