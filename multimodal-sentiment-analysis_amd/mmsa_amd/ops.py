@@ -1145,10 +1145,18 @@ def _matrices(ts, dtype, name):
     return ptrs
 
 
+# of one matrix; checked here too, as the library takes sizes as ints, which hold the low 32 bits of anything larger
+MAX_SIDE, MAX_VALUES = 2 ** 20, 2 ** 31
+
+
 def _sizes(ts):
     n = len(ts)
     rows = [t.shape[0] for t in ts]
-    return (ctypes.c_int * n)(*rows), (ctypes.c_int * n)(*[t.numel() // r for t, r in zip(ts, rows)])
+    cols = [t.numel() // r for t, r in zip(ts, rows)]
+    for t, r, c in zip(ts, rows, cols):
+        if r > MAX_SIDE or c > MAX_SIDE or r * c > MAX_VALUES:
+            raise _lib.MmsaError(f"matrix limit exceeded: {tuple(t.shape)} is more than 2^20 rows or columns or 2^31 values")
+    return (ctypes.c_int * n)(*rows), (ctypes.c_int * n)(*cols)
 
 
 def _ns_args(steps, eps):
@@ -1178,6 +1186,7 @@ def orthogonalize(srcs, dsts=None, steps: int = 5, eps: float = 1e-7):
         raise ValueError("orthogonalize: matrices [rows, cols]")
     n = len(srcs)
     src = _matrices(srcs, dtype, "orthogonalize")
+    rows, cols = _sizes(srcs)
     if dsts is None:
         dsts = [torch.empty_like(t) for t in srcs]
         dst = [t.data_ptr() for t in dsts]
@@ -1185,7 +1194,6 @@ def orthogonalize(srcs, dsts=None, steps: int = 5, eps: float = 1e-7):
         dst = _matrices(dsts, dtype, "orthogonalize")
         if dsts[0].device != srcs[0].device:
             raise ValueError("orthogonalize: the matrices of one call live on one device")
-    rows, cols = _sizes(srcs)
     stream = _stream()
     _lib.call("mmsa_orthogonalize", _parr(src), _parr(dst), rows, cols, n, DTYPE_CODES[dtype], int(steps), eps,
               _ns_scratch(rows, cols, n, srcs[0].device).data_ptr(), stream)
