@@ -890,7 +890,7 @@ __device__ __forceinline__ void wave_meet() {
 template <typename T, bool MOM, int NT>
 __global__ __launch_bounds__(512) void small_kernel(const Group gr, float mu, float one_minus_mu, int nesterov,
                                                     float eps, int steps, float decay, float rate) {
-  extern __shared__ unsigned words[];
+  extern __shared__ __attribute__((aligned(16))) unsigned words[];      // read four at a time
   __shared__ double red[16];
   const Mat q = gr.mat[blockIdx.x];
   const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, col = lane & 31, half = lane >> 5;

@@ -904,7 +904,7 @@ __global__ __launch_bounds__(1024) void gn_slab_fwd_kernel(const T* __restrict__
                                                            const float* __restrict__ beta, T* __restrict__ y,
                                                            double* __restrict__ stats, float eps, int act,
                                                            const Slab q) {
-  __shared__ float2 red[1024];
+  __shared__ __attribute__((aligned(16))) float2 red[1024];      // read as double2 too
   __shared__ double sum[GN_MAX_BUNDLE][2];
   const Place p = place_of(q);
   const int tid = threadIdx.x, col = tid % q.nw, r0 = tid / q.nw;
