@@ -35,7 +35,7 @@ constexpr float NS_A = 3.4445f, NS_C = 2.0315f;
 constexpr float NS_SHIFT = (float)(-4.775 / (2.0 * 2.0315)), NS_REST = (float)(3.4445 - 4.775 * 4.775 / (4.0 * 2.0315));
 constexpr int NS_SCALE = 14;           // log2 of the fixed-point scale
 constexpr int MAX_STEPS = 16;
-constexpr int GROUP = 24;              // matrices of one launch (their descriptors travel as kernel arguments)
+constexpr int GROUP = 24;              // matrices of one launch at most (their descriptors travel as kernel arguments)
 
 enum { PH_SUMSQ = 0, PH_SPLIT = 1, PH_PRODUCT = 2 /* T, B, X */, PH_JOIN = 5 /* T, B */, PH_COUNT = 7 };
 
@@ -1107,6 +1107,24 @@ int check_sizes(const int* rows, const int* cols, int count) {
   return MMSA_OK;
 }
 
+// How many of a list's next matrices share one set of launches: as many as their descriptors fit, up to a scratch of 1 GiB
+// (in the largest padding).  That is four rounds of 256 x 256 tiles on every compute unit, beyond which company gains
+// nothing (a single 4096 x 14336 matrix has 896 tiles); 24 of those together would ask for 20 GB.
+constexpr long SET_BYTES = 1l << 30;
+int set_of(const int* rows, const int* cols, int left) {
+  long bytes = 0;
+  int n = 0;
+  for (; n < left && n < GROUP; ++n) {
+    const int m = rows[n] < cols[n] ? rows[n] : cols[n], k = rows[n] < cols[n] ? cols[n] : rows[n];
+    Mat q;
+    q.mp = (m + 255) & ~255;
+    q.np = (k + 255) & ~255;
+    bytes += mat_bytes(q);
+    if (n && bytes > SET_BYTES) break;
+  }
+  return n;
+}
+
 struct Plan {
   int bt[3];       // tile of the T, B and X products
   int from[GROUP];   // which of the caller's matrices each one is
@@ -1349,10 +1367,11 @@ int launch_small(const Group& gr, const Step& st, hipStream_t s) {
 template <typename T, bool MOM>
 int run_all(const void* const* src, void* const* dst, void* const* mom, const int* rows, const int* cols, int count,
             const Step& st, void* scratch, hipStream_t s) {
-  for (int i0 = 0; i0 < count; i0 += GROUP) {
+  for (int i0 = 0, n; i0 < count; i0 += n) {
+    n = set_of(rows + i0, cols + i0, count - i0);
     Group gr;
     memset(&gr, 0, sizeof(gr));
-    gr.count = count - i0 < GROUP ? count - i0 : GROUP;
+    gr.count = n;
     Plan pl;
     make_plan(rows + i0, cols + i0, &gr, &pl);
     constexpr int NT_MOST = MOM ? 2 : 3;
@@ -1408,9 +1427,10 @@ bool pointers_ok(const void* const* p, int count) {
 MMSA_EXPORT long mmsa_orthogonalize_scratch_bytes(const int* rows_host, const int* cols_host, int count) {
   if (int rc = check_sizes(rows_host, cols_host, count)) return rc;
   long most = 0;
-  for (int i0 = 0; i0 < count; i0 += GROUP) {
+  for (int i0 = 0, n; i0 < count; i0 += n) {
+    n = set_of(rows_host + i0, cols_host + i0, count - i0);
     Group gr;
-    gr.count = count - i0 < GROUP ? count - i0 : GROUP;
+    gr.count = n;
     Plan pl;
     make_plan(rows_host + i0, cols_host + i0, &gr, &pl);
     if (pl.bytes > most) most = pl.bytes;

@@ -15,6 +15,68 @@ U = 2.0 ** -24
 A, B, C = 3.4445, -4.775, 2.0315
 
 
+def ns64(u, steps=5, eps=1e-7):
+    x = u.double()
+    x = x / max(float(x.norm()), eps)
+    tall = x.shape[0] > x.shape[1]
+    x = x.T.contiguous() if tall else x
+    for _ in range(steps):
+        s = x @ x.T
+        x = A * x + (B * s + C * (s @ s)) @ x
+    return x.T if tall else x
+
+
+def tol(shape, dtype=torch.float32):
+    return 31 * U * (4 + max(shape) ** 0.5 / 2) + (torch.finfo(dtype).eps / 2 if dtype != torch.float32 else U)
+
+
+def grad(m, n, seed=0, dtype=torch.float32):
+    g = torch.Generator(device=DEV).manual_seed(seed)
+    k = max(1, min(m, n) // 4)
+    low = torch.randn(m, k, device=DEV, generator=g) @ torch.randn(k, n, device=DEV, generator=g) / k ** 0.5
+    return ((low + 0.2 * torch.randn(m, n, device=DEV, generator=g)) * 1e-3).to(dtype)
+
+
+def close(got, want, rel):
+    d = got.double() - want
+    assert bool(torch.isfinite(got).all())
+    assert float(d.norm()) <= rel * float(want.norm()), (float(d.norm()) / float(want.norm()), rel)
+    # no single place stands out: 16 times a place's share of the whole
+    assert float(d.abs().max()) <= rel * (16 * float(want.norm()) / want.numel() ** 0.5 + float(want.abs().max()))
+
+
+def scratch_bytes(shapes):
+    from mmsa_amd import ops
+    n = len(shapes)
+    return ops._lib.query("mmsa_orthogonalize_scratch_bytes", ops._iarr([s[0] for s in shapes]),
+                          ops._iarr([s[1] for s in shapes]), n)
+
+
+def test_the_scratch_of_a_list_is_bounded():
+    """A list of large matrices is worked off in sets of launches that fill the chip, not all at once."""
+    one = scratch_bytes([(4096, 14336)])
+    assert scratch_bytes([(4096, 14336)] * 24) <= one + 2 ** 30 + 2 ** 20
+    assert scratch_bytes([(4096, 4096)] * 100) <= 2 ** 31
+    small = scratch_bytes([(256, 1152)])
+    assert 20 * small < scratch_bytes([(256, 1152)] * 24) < 30 * small         # these still go together
+
+
+@pytest.mark.gpu
+def test_lists_of_large_matrices():
+    """More than one set of launches because of their size, with small ones between them."""
+    from mmsa_amd.muon import muon_step, orthogonalize
+    shapes = [(2048, 8192), (70, 200), (4096, 4100), (4096, 4096), (33, 64), (2048, 8192), (130, 40)]
+    gs = [grad(*s, seed=i) for i, s in enumerate(shapes)]
+    wants = [ns64(g) for g in gs]
+    for s, o, w in zip(shapes, orthogonalize(gs), wants):
+        close(o, w, tol(s))
+    ps, ms = [torch.zeros_like(g) for g in gs], [g.clone() for g in gs]
+    muon_step(ps, gs, ms, lr=0.5)
+    for s, p, w in zip(shapes, ps, wants):
+        rate = 0.5 * max(1.0, s[0] / s[1]) ** 0.5
+        close(p, -rate * w, tol(s) + 31 * 8 * U)
+
+
 def test_sizes_that_32_bits_cannot_hold_are_refused():
     from mmsa_amd import _lib, ops
     for shape in ((2 ** 32 + 64, 64), (64, 2 ** 32 + 64), (2 ** 16, 2 ** 16), (2 ** 20 + 1, 2), (1, 2 ** 20 + 1)):
