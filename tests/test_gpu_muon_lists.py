@@ -45,6 +45,42 @@ def close(got, want, rel):
     assert float(d.abs().max()) <= rel * (16 * float(want.norm()) / want.numel() ** 0.5 + float(want.abs().max()))
 
 
+# sizes for which the general product comes in tiles of 128 and of 256, wide and tall, neither side a multiple of a tile
+LARGE = [(2000, 2101), (2101, 2000), (2500, 4999), (4999, 2500)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16], ids=str)
+@pytest.mark.parametrize("shape", LARGE, ids=str)
+def test_large_tiles_in_every_type(shape, dtype):
+    from mmsa_amd.muon import orthogonalize
+    g = grad(*shape, seed=sum(shape), dtype=dtype)
+    o = orthogonalize(g)
+    want = ns64(g)
+    close(o, want, tol(shape, dtype))
+    if dtype != torch.float32:
+        # every place is the rounding of a value that float32 products leave near the exact one
+        near = tol(shape) * (16 * float(want.norm()) / want.numel() ** 0.5 + want.abs())
+        half = torch.finfo(dtype).eps / 2 * (want.abs() + near) + torch.finfo(dtype).tiny * torch.finfo(dtype).eps / 2
+        assert bool(((o.double() - want).abs() <= near + half).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("shape", LARGE, ids=str)
+def test_large_tiles_into_a_parameter(shape):
+    from mmsa_amd.muon import muon_step
+    p, g, m = torch.randn(shape, device=DEV) * 0.02, grad(*shape, seed=1), grad(*shape, seed=2)
+    p0, mom = p.double(), m.double() + (1 - 0.95) * (g.double() - m.double())
+    o = ns64(g.double() + 0.95 * (mom - g.double()))
+    rate = 0.02 * max(1.0, shape[0] / shape[1]) ** 0.5
+    want = p0 * (1 - 0.02 * 0.1) - rate * o
+    muon_step([p], [g], [m], lr=0.02, weight_decay=0.1)
+    assert float((m.double() - mom).abs().max()) <= 4 * U * float(mom.abs().max() + g.abs().max())
+    # the direction is known to a few u, which the iteration magnifies 31 times; the parameter is rounded three times
+    bound = rate * (tol(shape) + 31 * 8 * U) * float(o.norm()) + 4 * U * float(p0.norm())
+    assert float((p.double() - want).norm()) <= bound
+
+
 def scratch_bytes(shapes):
     from mmsa_amd import ops
     n = len(shapes)
