@@ -44,8 +44,8 @@ def muon_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], mom
     ``m += (1 - momentum)(g - m);  u = g + momentum (m - g) if nesterov else m;``
     ``p = p (1 - lr weight_decay) - lr sqrt(max(1, rows / cols)) orthogonalize(u)``
 
-    A tensor of more than two dimensions is taken as [first, rest].  Parameters and momenta are contiguous and no two of
-    them share memory.  The scalars are held by value: a step captured in a HIP graph replays with those of the capture.
+    A tensor of more than two dimensions is taken as [first, rest].  Parameters and momenta are contiguous and share no
+    memory with each other or with a gradient.  The scalars are held by value: a step captured in a HIP graph replays with those of the capture.
     """
     ops.muon_step(params, [g if g.is_contiguous() else g.contiguous() for g in grads], momenta, lr, weight_decay,
                   momentum, nesterov, steps, eps)

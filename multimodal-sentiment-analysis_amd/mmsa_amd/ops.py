@@ -1159,6 +1159,22 @@ def _sizes(ts):
     return (ctypes.c_int * n)(*rows), (ctypes.c_int * n)(*cols)
 
 
+def _apart(written, read, what):
+    """Refuses operands, as (address, tensor), of which one that is written shares memory with another."""
+    writes, reads = ([(a, a + t.nbytes) for a, t in ts] for ts in (written, read))
+    spans = sorted(writes + reads)
+    if all(x[1] <= y[0] for x, y in zip(spans, spans[1:])):
+        return
+    writes = set(writes)                 # (two equal ones of these are found below, being two spans)
+    write_end = any_end = 0
+    for span in spans:
+        if span[0] < (any_end if span in writes else write_end):
+            raise ValueError(f"{what} is listed twice or shares memory with another operand")
+        any_end = max(any_end, span[1])
+        if span in writes:
+            write_end = any_end
+
+
 def _ns_args(steps, eps):
     if not 1 <= int(steps) <= 16 or int(steps) != steps:
         raise ValueError("steps must be a whole number from 1 to 16")
@@ -1194,6 +1210,7 @@ def orthogonalize(srcs, dsts=None, steps: int = 5, eps: float = 1e-7):
         dst = _matrices(dsts, dtype, "orthogonalize")
         if dsts[0].device != srcs[0].device:
             raise ValueError("orthogonalize: the matrices of one call live on one device")
+        _apart(zip(dst, dsts), [(a, t) for a, t, d in zip(src, srcs, dst) if a != d], "orthogonalize: a destination")
     stream = _stream()
     _lib.call("mmsa_orthogonalize", _parr(src), _parr(dst), rows, cols, n, DTYPE_CODES[dtype], int(steps), eps,
               _ns_scratch(rows, cols, n, srcs[0].device).data_ptr(), stream)
@@ -1202,7 +1219,7 @@ def orthogonalize(srcs, dsts=None, steps: int = 5, eps: float = 1e-7):
 
 def muon_step(params, grads, momenta, lr, weight_decay, momentum, nesterov=True, steps: int = 5, eps: float = 1e-7):
     """One Muon step over contiguous fp32 tensors, each taken as a matrix [first, rest]; params and momenta are updated in
-    place (no two share memory)."""
+    place (they share no memory with each other or with a gradient)."""
     _ns_args(steps, eps)
     if not len(params) == len(grads) == len(momenta) or any(p.shape != g.shape or p.shape != m.shape
                                                             for p, g, m in zip(params, grads, momenta)):
@@ -1213,9 +1230,7 @@ def muon_step(params, grads, momenta, lr, weight_decay, momentum, nesterov=True,
     ptrs = [_matrices(ts, F32, name) for ts, name in ((params, "params"), (grads, "grads"), (momenta, "momenta"))]
     if not params[0].device == grads[0].device == momenta[0].device:
         raise ValueError("muon_step: the matrices of one call live on one device")
-    written = {*ptrs[0], *ptrs[2]}
-    if len(written) != 2 * n or not written.isdisjoint(ptrs[1]):
-        raise ValueError("muon_step: a parameter or momentum buffer is listed twice")
+    _apart([*zip(ptrs[0], params), *zip(ptrs[2], momenta)], zip(ptrs[1], grads), "muon_step: a parameter or momentum buffer")
     rows, cols = _sizes(params)
     stream = _stream()
     _lib.call("mmsa_muon_step", *map(_parr, ptrs), rows, cols, n, float(lr), float(weight_decay), float(momentum), int(nesterov),

@@ -120,3 +120,47 @@ def test_sizes_that_32_bits_cannot_hold_are_refused():
             ops._sizes([torch.empty(4, 4, device="meta"), torch.empty(shape, device="meta")])
     rows, cols = ops._sizes([torch.empty(2 ** 20, 2 ** 11, device="meta"), torch.empty(8, 4, 3, 3, device="meta")])
     assert list(rows) == [2 ** 20, 8] and list(cols) == [2 ** 11, 36]
+
+
+@pytest.mark.gpu
+def test_operands_that_share_memory_are_refused():
+    from mmsa_amd import ops
+    from mmsa_amd.muon import muon_step
+    flat = torch.zeros(64, 8, device=DEV)
+    a, over, apart = flat[:32], flat[31:63], torch.zeros(32, 8, device=DEV)
+    g, m, n = (torch.zeros(32, 8, device=DEV) for _ in range(3))
+    for args in (([a, over], [g, g], [m, n]), ([a], [over], [m]), ([a], [g], [over]), ([m, n], [g, g], [a, over])):
+        with pytest.raises(ValueError, match="share"):
+            muon_step(*args, lr=0.1)
+    for srcs, dsts in (([a, apart], [m, m]), ([a, apart], [apart, m]), ([a], [over])):
+        with pytest.raises(ValueError, match="share"):
+            ops.orthogonalize(srcs, dsts)
+    ops.orthogonalize([a, apart], [a, m])                   # in its own place
+    muon_step([flat[:32], flat[32:]], [g, g], [m, n], lr=0.1)          # neighbours, one gradient for both
+
+
+def test_the_check_for_shared_memory_against_every_pair():
+    import random
+
+    from mmsa_amd import ops
+    memory, rng = torch.zeros(4000), random.Random(1)
+
+    def some(k):
+        at = [rng.randrange(3000) for _ in range(k)]
+        return [(t.data_ptr(), t) for t in (memory[a:a + rng.randrange(1, 400)] for a in at)]
+
+    def meet(x, y):
+        return x[0] < y[0] + y[1].nbytes and y[0] < x[0] + x[1].nbytes
+    refused = 0
+    for _ in range(2000):
+        writes, reads = some(rng.randrange(4)), some(rng.randrange(4))
+        if writes and reads and rng.random() < 0.2:
+            reads[0] = writes[0]
+        want = any(meet(x, y) for i, x in enumerate(writes) for y in writes[:i] + reads)
+        try:
+            ops._apart(writes, reads, "a tensor")
+            assert not want
+        except ValueError as e:
+            assert want and "share" in str(e)
+            refused += 1
+    assert 200 < refused < 1800
