@@ -82,21 +82,27 @@ class Muon(torch.optim.Optimizer):
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
+        todo = []                       # every group is checked before the first one is updated
         for group in self.param_groups:
+            ops._ns_args(group["steps"], group["eps"])
             by_device: dict = {}
             for p in group["params"]:
                 if p.grad is None:
                     continue
                 if p.grad.is_sparse:
                     raise RuntimeError("Muon does not take sparse gradients")
+                _gpu([p], "Muon")
+                if not p.is_contiguous():
+                    raise ValueError(f"Muon: parameters must be contiguous, one of {tuple(p.shape)} is not")
+                by_device.setdefault(p.device, []).append(p)
+            todo += [(group, device, ps) for device, ps in by_device.items()]
+        for group, device, ps in todo:
+            for p in ps:
                 state = self.state[p]
                 if "momentum_buffer" not in state:
                     state["momentum_buffer"] = torch.zeros_like(p, memory_format=torch.contiguous_format)
-                by_device.setdefault(p.device, []).append((p, p.grad, state["momentum_buffer"]))
-            for device, triples in by_device.items():
-                _gpu([triples[0][0]], "Muon")
-                with torch.cuda.device(device):
-                    muon_step(*zip(*triples), lr=float(group["lr"]), weight_decay=group["weight_decay"],
-                              momentum=group["momentum"], nesterov=group["nesterov"], steps=group["steps"],
-                              eps=group["eps"])
+            with torch.cuda.device(device):
+                muon_step(ps, [p.grad for p in ps], [self.state[p]["momentum_buffer"] for p in ps],
+                          lr=float(group["lr"]), weight_decay=group["weight_decay"], momentum=group["momentum"],
+                          nesterov=group["nesterov"], steps=group["steps"], eps=group["eps"])
         return loss

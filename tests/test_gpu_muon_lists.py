@@ -164,3 +164,31 @@ def test_the_check_for_shared_memory_against_every_pair():
             assert want and "share" in str(e)
             refused += 1
     assert 200 < refused < 1800
+
+
+def _params(*shapes):
+    gen = torch.Generator(device=DEV).manual_seed(7)
+    ps = [torch.nn.Parameter(torch.randn(s, device=DEV, generator=gen)) for s in shapes]
+    for p in ps:
+        p.grad = torch.randn(p.shape, device=DEV, generator=gen)
+    return ps
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bad", ["cpu", "sparse", "order"])
+def test_a_refused_step_leaves_everything_as_it_was(bad):
+    from mmsa_amd import _lib
+    from mmsa_amd.muon import Muon
+    good, q = _params((8, 8), (8, 4, 3, 3))
+    if bad == "cpu":
+        q = torch.nn.Parameter(torch.randn(8, 36))
+        q.grad = torch.randn(8, 36)
+    opt = Muon([{"params": [good]}, {"params": [q]}], lr=0.1)
+    if bad == "sparse":
+        q.grad = torch.zeros(8, 4, 3, 3, device=DEV).to_sparse()
+    if bad == "order":
+        q.data = q.data.to(memory_format=torch.channels_last)
+    before = good.detach().clone()
+    with pytest.raises((_lib.MmsaError, RuntimeError, ValueError)):
+        opt.step()
+    assert torch.equal(good, before) and not opt.state
