@@ -54,7 +54,7 @@ def muon_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], mom
 
 
 class Muon(torch.optim.Optimizer):
-    """Muon over float32 weight matrices on the GPU, as a ``torch.optim.Optimizer``: the reference's loop
+    """Muon over contiguous float32 weight matrices on the GPU, as a ``torch.optim.Optimizer``: the reference's loop
     (`multimodal_train.py:175-195`), its schedulers and ``state_dict`` work on it unchanged.
 
     Only parameters with at least two dimensions are taken (pass the others to ``torch.optim.AdamW``); a parameter
@@ -71,10 +71,10 @@ class Muon(torch.optim.Optimizer):
     def add_param_group(self, param_group):
         super().add_param_group(param_group)
         for p in self.param_groups[-1]["params"]:
-            if p.dim() < 2 or p.dtype != torch.float32:
+            if p.dim() < 2 or p.dtype != torch.float32 or not p.is_contiguous():
                 self.param_groups.pop()
-                raise ValueError("Muon takes float32 parameters with at least two dimensions, got "
-                                 f"{p.dtype} {tuple(p.shape)}")
+                raise ValueError("Muon takes contiguous float32 parameters with at least two dimensions, got "
+                                 f"{p.dtype} {tuple(p.shape)} with strides {p.stride()}")
 
     @torch.no_grad()
     def step(self, closure=None):

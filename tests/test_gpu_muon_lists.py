@@ -192,3 +192,17 @@ def test_a_refused_step_leaves_everything_as_it_was(bad):
     with pytest.raises((_lib.MmsaError, RuntimeError, ValueError)):
         opt.step()
     assert torch.equal(good, before) and not opt.state
+
+
+@pytest.mark.gpu
+def test_parameters_in_another_order_are_refused_when_they_are_given():
+    from mmsa_amd.muon import Muon
+    good, q = _params((8, 8), (8, 4, 3, 3))
+    q.data = q.data.to(memory_format=torch.channels_last)
+    with pytest.raises(ValueError, match="contiguous"):
+        Muon([good, q])
+    opt = Muon([good])
+    with pytest.raises(ValueError, match="contiguous"):
+        opt.add_param_group({"params": [q]})
+    opt.step()
+    assert len(opt.param_groups) == 1
