@@ -58,7 +58,7 @@ class Muon(torch.optim.Optimizer):
     (`multimodal_train.py:175-195`), its schedulers and ``state_dict`` work on it unchanged.
 
     Only parameters with at least two dimensions are taken (pass the others to ``torch.optim.AdamW``); a parameter
-    without a gradient is left alone.  All matrices of a group are updated in shared launches."""
+    without a gradient, or without values, is left alone.  All matrices of a group are updated in shared launches."""
 
     def __init__(self, params, lr: float = 0.02, weight_decay: float = 0.0, momentum: float = 0.95,
                  nesterov: bool = True, steps: int = 5, eps: float = 1e-7):
@@ -87,7 +87,7 @@ class Muon(torch.optim.Optimizer):
             ops._ns_args(group["steps"], group["eps"])
             by_device: dict = {}
             for p in group["params"]:
-                if p.grad is None:
+                if p.grad is None or not p.numel():
                     continue
                 if p.grad.is_sparse:
                     raise RuntimeError("Muon does not take sparse gradients")

@@ -206,3 +206,12 @@ def test_parameters_in_another_order_are_refused_when_they_are_given():
         opt.add_param_group({"params": [q]})
     opt.step()
     assert len(opt.param_groups) == 1
+
+
+@pytest.mark.gpu
+def test_an_empty_parameter_is_left_alone():
+    from mmsa_amd.muon import Muon
+    good, empty = _params((8, 8), (0, 4))
+    before = good.detach().clone()
+    Muon([good, empty], lr=0.1).step()
+    assert not torch.equal(good, before) and empty.shape == (0, 4)
