@@ -58,7 +58,8 @@ class Muon(torch.optim.Optimizer):
     (`multimodal_train.py:175-195`), its schedulers and ``state_dict`` work on it unchanged.
 
     Only parameters with at least two dimensions are taken (pass the others to ``torch.optim.AdamW``); a parameter
-    without a gradient, or without values, is left alone.  All matrices of a group are updated in shared launches."""
+    without a gradient, or without values, is left alone.  All matrices of a group are updated in shared launches.  A step
+    can be captured in a HIP graph once every parameter has had an eager one."""
 
     def __init__(self, params, lr: float = 0.02, weight_decay: float = 0.0, momentum: float = 0.95,
                  nesterov: bool = True, steps: int = 5, eps: float = 1e-7):
@@ -94,6 +95,9 @@ class Muon(torch.optim.Optimizer):
                 _gpu([p], "Muon")
                 if not p.is_contiguous():
                     raise ValueError(f"Muon: parameters must be contiguous, one of {tuple(p.shape)} is not")
+                if "momentum_buffer" not in self.state.get(p, ()) and torch.cuda.is_current_stream_capturing():
+                    raise RuntimeError("Muon makes its momentum at a parameter's first step, which has to be an eager "
+                                       "one: cleared inside a graph, it would be cleared again by every replay")
                 by_device.setdefault(p.device, []).append(p)
             todo += [(group, device, ps) for device, ps in by_device.items()]
         for group, device, ps in todo:

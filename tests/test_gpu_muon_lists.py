@@ -215,3 +215,33 @@ def test_an_empty_parameter_is_left_alone():
     before = good.detach().clone()
     Muon([good, empty], lr=0.1).step()
     assert not torch.equal(good, before) and empty.shape == (0, 4)
+
+
+@pytest.mark.gpu
+def test_momentum_is_not_made_inside_a_graph():
+    """A buffer made and cleared while a graph is recorded would be cleared again by every replay: the first step is an
+    eager one, and replays then follow eager steps."""
+    from mmsa_amd.muon import Muon
+    ps, qs = _params((48, 80), (7, 300)), _params((48, 80), (7, 300))
+    opt, ref = Muon(ps, lr=0.02), Muon(qs, lr=0.02)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.stream(side), pytest.raises(RuntimeError, match="eager"):
+        with torch.cuda.graph(graph, stream=side, capture_error_mode="thread_local"):
+            opt.step()
+    torch.cuda.synchronize()
+    assert not opt.state and all(torch.equal(p, q) for p, q in zip(ps, qs))
+    opt.step()
+    ref.step()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, capture_error_mode="thread_local"):
+        opt.step()
+    for k in range(4):
+        for p, q in zip(ps, qs):
+            p.grad.normal_()
+            q.grad.copy_(p.grad)
+        graph.replay()
+        ref.step()
+        torch.cuda.synchronize()
+        assert all(torch.equal(p, q) for p, q in zip(ps, qs)), k
