@@ -96,7 +96,8 @@ def group_norm_act(x: torch.Tensor, num_groups: int, weight=None, bias=None, eps
 
 class GroupNormAct(nn.Module):
     """``torch.nn.GroupNorm`` followed by an activation as one operator: same constructor order, parameters and
-    ``state_dict`` keys (``weight``, ``bias``) as ``nn.GroupNorm``; see :func:`group_norm_act`."""
+    ``state_dict`` keys (``weight``, ``bias``) as ``nn.GroupNorm``; see :func:`group_norm_act`.  A module converted to
+    16 bits keeps its parameters in that type and computes with their float32 values."""
 
     def __init__(self, num_groups: int, num_channels: int, eps: float = 1e-5, affine: bool = True,
                  activation: str = "relu"):
@@ -112,7 +113,10 @@ class GroupNormAct(nn.Module):
     def forward(self, x):
         if x.dim() < 2 or x.shape[1] != self.num_channels:
             raise ValueError(f"GroupNormAct({self.num_groups}, {self.num_channels}) got a map of shape {tuple(x.shape)}")
-        return group_norm_act(x, self.num_groups, self.weight, self.bias, self.eps, self.activation)
+        # the kernels take float32 parameters; those of a module converted to 16 bits are widened (C values each)
+        weight, bias = (p if p is None or p.dtype not in (torch.bfloat16, torch.float16) else p.float()
+                        for p in (self.weight, self.bias))
+        return group_norm_act(x, self.num_groups, weight, bias, self.eps, self.activation)
 
     def extra_repr(self):
         return (f"{self.num_groups}, {self.num_channels}, eps={self.eps}, affine={self.weight is not None}, "

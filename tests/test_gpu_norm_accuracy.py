@@ -121,6 +121,30 @@ def test_forward_mode_tangents_are_refused():
     assert y.requires_grad
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=str)
+def test_a_module_converted_to_16_bits(dtype):
+    """model.to(bfloat16) converts the parameters too: they are taken at their values, and their gradients come in their
+    type."""
+    from mmsa_amd.norm import GroupNormAct, group_norm_act
+    torch.manual_seed(3)
+    m = GroupNormAct(4, 24, activation="silu").to(DEV)
+    with torch.no_grad():
+        m.weight.normal_(1, 0.2)
+        m.bias.normal_(0, 0.2)
+    m.to(dtype)
+    x = torch.randn(3, 24, 7, 9, device=DEV, dtype=dtype, requires_grad=True)
+    dy = torch.randn(3, 24, 7, 9, device=DEV, dtype=dtype)
+    w, b = (p.detach().float().requires_grad_() for p in (m.weight, m.bias))
+    want = group_norm_act(x, 4, w, b, 1e-5, "silu")
+    got = m(x)
+    assert got.dtype == dtype and torch.equal(got, want)
+    for g, v in zip(torch.autograd.grad(got, (x, m.weight, m.bias), dy), torch.autograd.grad(want, (x, w, b), dy)):
+        assert g.dtype == dtype and torch.equal(g, v.to(dtype))
+    with pytest.raises(TypeError):                       # 64 bits would be narrowed
+        m.double()(x)
+
+
 def test_channel_counts_that_32_bits_cannot_hold_are_refused():
     from mmsa_amd import _lib, ops
     for C in (2 ** 31, 2 ** 32 + 8):
