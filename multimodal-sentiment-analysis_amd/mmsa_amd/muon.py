@@ -3,7 +3,10 @@
 The reference trains every parameter with ``torch.optim.AdamW`` (`CNN implementation/multimodal_train.py:481-485`).  The
 Muon rule gives the weight MATRICES (convolutions flattened to [out, in * taps], linear layers) another update: momentum,
 then the nearest matrix with all singular values near 1, so that no direction of the gradient dominates the step.
-Biases, norms, embeddings and the classifier stay with AdamW.
+Biases, norms, the embedding and the classifier's last layer stay with AdamW.
+
+The rule and the coefficients of its iteration are K. Jordan and others', "Muon: an optimizer for hidden layers in neural
+networks" (2024).
 """
 from __future__ import annotations
 
@@ -26,7 +29,8 @@ def orthogonalize(matrices: Union[torch.Tensor, Sequence[torch.Tensor]], steps: 
     ``X = u / max(|u|_F, eps)``, then ``steps`` times ``X <- (a I + b S + c S S) X`` with ``S = X X^T`` (on the transpose
     where rows exceed columns) and (a, b, c) = (3.4445, -4.775, 2.0315): singular values that are not tiny end between 0.7
     and 1.2.  float32, bfloat16 or float16 in and out (one type per list), computed to float32 accuracy.  Returns new
-    contiguous tensors; no gradient flows through.  A list may hold matrices of different sizes.
+    contiguous tensors; no gradient flows through.  A list may hold matrices of different sizes: tiles and splits are
+    chosen for all that share a launch, so a matrix's last bits can depend on its company.
     """
     single = isinstance(matrices, torch.Tensor)
     ms = [matrices] if single else list(matrices)

@@ -245,3 +245,47 @@ def test_momentum_is_not_made_inside_a_graph():
         ref.step()
         torch.cuda.synchronize()
         assert all(torch.equal(p, q) for p, q in zip(ps, qs)), k
+
+
+@pytest.mark.gpu
+def test_muon_and_adamw_train_the_model_together():
+    """The package's own model: its hidden weight matrices with Muon, the embedding, the classifier's last layer and all
+    vectors with AdamW; every parameter is updated once, by its own rule, over steps with changing gradients.
+
+    Some of these gradients have a low rank (the two rows of the attention over two modalities are opposite), and what
+    lies in their empty directions grows by a = 3.4445 in every step.  A rounding of the iteration is magnified at most
+    1 + a + ... + a^4 = 198 times there, one of the direction a^5 = 485 times.  The direction's own: every step rounds the
+    factor 1 - momentum, g - m and m; then the factor momentum, m - g and u are rounded."""
+    from conftest import SMALL_VOCAB, batch_tensors, model_inputs, seeded_model
+    from mmsa_amd.muon import Muon
+    m = seeded_model("both", vocab=SMALL_VOCAB).to(DEV).train()
+    apart = {m.text_model.embedding.weight, m.classifier[-1].weight}
+    matrices = [p for p in m.parameters() if p.dim() >= 2 and p not in apart]
+    others = [p for p in m.parameters() if p.dim() < 2 or p in apart]
+    assert len(matrices) == 24 and len(matrices) + len(others) == len(list(m.parameters()))
+    opts = [Muon(matrices, lr=0.02, weight_decay=0.01), torch.optim.AdamW(others, lr=1e-3)]
+    mom = [torch.zeros_like(p, dtype=torch.float64) for p in matrices]
+    most_g, most_m = [0.0] * len(matrices), [0.0] * len(matrices)
+    for it in range(3):
+        b = batch_tensors(8 * it, 8, vocab=SMALL_VOCAB, device=DEV)
+        for o in opts:
+            o.zero_grad()
+        m(**model_inputs("both", b), labels=b["label"])["loss"].backward()
+        before = [p.detach().double() for p in matrices]
+        rest = [p.detach().clone() for p in others]
+        for o in opts:
+            o.step()
+        for k, (p, p0) in enumerate(zip(matrices, before)):
+            g = p.grad.double()
+            mom[k] = mom[k] + (1 - 0.95) * (g - mom[k])
+            most_g[k], most_m[k] = max(most_g[k], float(g.norm())), max(most_m[k], float(mom[k].norm()))
+            rows, cols = p.shape[0], p[0].numel()
+            u = g + 0.95 * (mom[k] - g)
+            o = ns64(u.view(rows, cols)).reshape(p.shape)
+            rate = 0.02 * max(1.0, rows / cols) ** 0.5
+            both, size = most_g[k] + most_m[k], float(u.norm())
+            direction = U * ((it + 1) * (0.1 * both + most_m[k]) + 2 * both + size) / size
+            iteration = 198 * U * (4 + max(rows, cols) ** 0.5 / 2) * max(1.0, float(o.norm()))
+            off = float((p.detach().double() - (p0 * (1 - 0.02 * 0.01) - rate * o)).norm())
+            assert off <= rate * (iteration + 485 * direction) + 4 * U * float(p0.norm()), (k, p.shape)
+        assert sum(not torch.equal(p, r) for p, r in zip(others, rest)) >= len(others) - 1
