@@ -464,8 +464,9 @@ MMSA_API int mmsa_group_norm_act_bwd(const void* dy, const void* x, const float*
  * matrices of one dtype (MMSA_F32 / MMSA_BF16 / MMSA_F16), row-major contiguous [rows][cols], in shared launches;
  * dst[i] may be src[i], apart from that no destination shares memory with another operand.  *_host: host arrays of
  * `count` device pointers / sizes.  1 <= steps <= 16.  A zero matrix gives zeros; a matrix holding an infinity or NaN
- * gives NaN, without touching the others.  Accuracy is that of fp32 products whatever the dtype.  Limits
- * (MMSA_ERR_LIMIT): 2^20 rows or columns, 2^31 values a matrix.
+ * gives NaN, without touching the others.  Operands are held to 2^-23, whatever the dtype, and summed in fp32: about as
+ * exact as fp32 products.  Matrices share launches as far as their scratch stays within 1 GiB (one matrix may need
+ * more).  Limits (MMSA_ERR_LIMIT): 2^20 rows or columns, 2^31 values a matrix.
  * scratch: mmsa_orthogonalize_scratch_bytes(...) bytes, 128-byte aligned. */
 MMSA_API long mmsa_orthogonalize_scratch_bytes(const int* rows_host, const int* cols_host, int count);
 MMSA_API int mmsa_orthogonalize(const void* const* src_host, void* const* dst_host, const int* rows_host,

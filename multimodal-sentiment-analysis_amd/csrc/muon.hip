@@ -9,11 +9,17 @@
 // Arithmetic.  x -> a x + b x^3 + c x^5 maps [0, 1.2025] into itself, so singular values, hence entries, of X never
 // exceed 1.2025, those of T 1.18 and those of B 3.4445: every operand fits ONE fixed power-of-two
 // scale of 2^14 in fp16, with no overflow for any input.  Each value is held as a pair hi = fp16(v), lo = fp16(v - hi),
-// which keeps 2^-24 relative (fp32's own half unit) down to 2^-39 absolute, and each product is three fp16 matrix
-// products hi hi + hi lo + lo hi into one fp32 accumulator; lo lo is below 2^-24 relative and left out.  That is fp32
-// accuracy at a third of the fp16 matrix rate (about 2.5 PFLOP/s) instead of the fp32 matrix rate (157 TFLOP/s).
+// which is within 2^-23 of it (one unit of fp32 in a quarter of all values, exact in the others) or 2^-39 absolutely,
+// and each product is three fp16 matrix products hi hi + hi lo + lo hi into fp32 accumulators.  lo lo is left out: at
+// most 2^-22 of a product, of either sign, except on the diagonals of X X^T and T T, where it is a square and leaves
+// them 2^-24.6 short in the mean.  Against 64 bits the result is off by 0.5 to 1.2 times what plain fp32 products leave
+// (1.4 with tiles of 256), at a third of the fp16 matrix rate (about 2.5 PFLOP/s) instead of the fp32 matrix rate (157
+// TFLOP/s).
 // A matrix whose norm is below eps enters with entries far below 1: its X is held at a larger scale 2^(14 + k), k from
 // the norm (the polynomial grows it by at most a per step, so k shrinks from step to step by the same bound).
+//
+// The rule and the coefficients are published: K. Jordan and others, "Muon: an optimizer for hidden layers in neural
+// networks" (2024).
 //
 // Layout.  A padded matrix [rows][K] of pairs is stored as [row][K / 16][hi 16 | lo 16] fp16: 16 values of a row, what
 // one matrix instruction takes, are 64 bytes holding both halves.  All products are row times row
@@ -364,7 +370,8 @@ struct Fragments {
 //
 // A matrix instruction rounds twice into its fp32 accumulator.  The products hi lo + lo hi are 2^-11 of hi hi: in an
 // accumulator of their own they round at that scale, and the main one is rounded a third as often (0.6 of the error at
-// K = 2048).  The 256 x 256 tile has no registers left for that.
+// K = 2048).  The 256 x 256 tile has no registers left for that: four 2048 x 2048 and a 2048 x 8192 end 1.2 to 1.4 times as
+// far from the exact result as plain fp32 products do.
 template <int BT>
 __device__ __forceinline__ void multiply(f32x16 (&acc)[Tile<BT>::W][Tile<BT>::W], char* lds, const char* P,
                                          const char* Q, long pitch, int nk32) {
