@@ -12,9 +12,9 @@
 // which is within 2^-23 of it (one unit of fp32 in a quarter of all values, exact in the others) or 2^-39 absolutely,
 // and each product is three fp16 matrix products hi hi + hi lo + lo hi into fp32 accumulators.  lo lo is left out: at
 // most 2^-22 of a product, of either sign, except on the diagonals of X X^T and T T, where it is a square and leaves
-// them 2^-24.6 short in the mean.  Against 64 bits the result is off by 0.5 to 1.2 times what plain fp32 products leave
-// (1.4 with tiles of 256), at a third of the fp16 matrix rate (about 2.5 PFLOP/s) instead of the fp32 matrix rate (157
-// TFLOP/s).
+// them 2^-24.6 short in the mean.  Against 64 bits the result is off by 0.5 to 1.3 times what plain fp32 products leave
+// (0.9 in the median of 151 matrices of 2 to 3000 rows; 1.4 with tiles of 256; for a handful of rows chance decides, up
+// to 2.3), at a third of the fp16 matrix rate (about 2.5 PFLOP/s) instead of the fp32 matrix rate (157 TFLOP/s).
 // A matrix whose norm is below eps enters with entries far below 1: its X is held at a larger scale 2^(14 + k), k from
 // the norm (the polynomial grows it by at most a per step, so k shrinks from step to step by the same bound).
 //

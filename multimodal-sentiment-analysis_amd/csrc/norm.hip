@@ -513,7 +513,8 @@ struct Channel {
 // 64 rows in 32 bits and adds them up in its place in LDS; threads and chunks are joined in 64 bits, their sums kept in
 // 32 in between.  4 x 16384 x 512 bf16, SiLU: 31 us, 134 MB at 4.3 TB/s; the vector unit is as busy as memory (the slope
 // of an activation is 12 to 20 instructions a value).
-template <typename T, int ACT, bool ONCE>
+// RUNS: chunks of more than one run; such maps are read past the cache anyway, and the others keep the registers.
+template <typename T, int ACT, bool ONCE, bool RUNS>
 __global__ __launch_bounds__(1024) void gn_bwd_sums_kernel(const T* __restrict__ dy, const T* __restrict__ x,
                                                            const float* __restrict__ gamma,
                                                            const float* __restrict__ beta,
@@ -535,7 +536,10 @@ __global__ __launch_bounds__(1024) void gn_bwd_sums_kernel(const T* __restrict__
     k.load(stats + 2 * b * cut.G, gamma, beta, (int)(((long)t * V) % cut.C), cut.C, cut.Cg);
     float s1[V], s2[V];           // sums of dz and of dz (x - mean)
 #pragma unroll
-    for (int e = 0; e < V; ++e) sh[t * V + e] = sh[slots + t * V + e] = s1[e] = s2[e] = 0.f;
+    for (int e = 0; e < V; ++e) {
+      s1[e] = s2[e] = 0.f;
+      if (RUNS) sh[t * V + e] = sh[slots + t * V + e] = 0.f;
+    }
     auto add = [&](int e, float v, float h) {
       float d;
       const float dz = k.template grad<ACT, Io<T>::FINE>(e, v, h, d);
@@ -546,14 +550,14 @@ __global__ __launch_bounds__(1024) void gn_bwd_sums_kernel(const T* __restrict__
     auto leave = [&]() {
 #pragma unroll
       for (int e = 0; e < V; ++e) {
-        sh[t * V + e] += s1[e];
-        sh[slots + t * V + e] += s2[e];
+        sh[t * V + e] = RUNS ? sh[t * V + e] + s1[e] : s1[e];
+        sh[slots + t * V + e] = RUNS ? sh[slots + t * V + e] + s2[e] : s2[e];
         s1[e] = s2[e] = 0.f;
       }
     };
     int it = 0;
     for (; it + U <= me.full; it += U, p += U * hop, g += U * hop) {
-      if (it && it % GN_RUN == 0) leave();
+      if (RUNS && it && it % GN_RUN == 0) leave();
       Pack<T, V> f[U], h[U];
 #pragma unroll
       for (int u = 0; u < U; ++u) {
@@ -1325,8 +1329,13 @@ int cut_bwd(const T* dy, const T* x, const float* gamma, const float* beta, cons
   float* coef = sums + batch * cut.C * 2;
   const dim3 grid((unsigned)(batch * cut.nchunk)), block(block_of(cut));
   const size_t lds = 2 * sizeof(float) * slots_of(cut, dtype);
-  if (int rc = allow_lds<gn_bwd_sums_kernel<T, ACT, ONCE>>(lds)) return rc;
-  hipLaunchKernelGGL((gn_bwd_sums_kernel<T, ACT, ONCE>), grid, block, lds, s, dy, x, gamma, beta, stats, cut, part);
+  if (ONCE && cut.iters > GN_RUN) {
+    if (int rc = allow_lds<gn_bwd_sums_kernel<T, ACT, true, true>>(lds)) return rc;
+    hipLaunchKernelGGL((gn_bwd_sums_kernel<T, ACT, true, true>), grid, block, lds, s, dy, x, gamma, beta, stats, cut, part);
+  } else {
+    if (int rc = allow_lds<gn_bwd_sums_kernel<T, ACT, ONCE, false>>(lds)) return rc;
+    hipLaunchKernelGGL((gn_bwd_sums_kernel<T, ACT, ONCE, false>), grid, block, lds, s, dy, x, gamma, beta, stats, cut, part);
+  }
   const int span = cut.Cg > 64 ? 64 : 64 / cut.Cg * cut.Cg;
   hipLaunchKernelGGL(gn_bwd_join_kernel, dim3((unsigned)(batch * mmsa_cdiv(cut.C, span))),
                      dim3(cut.nchunk < 64 ? 256 : 1024), 0, s, part, cut, span, gamma, sums, coef);
@@ -1357,7 +1366,7 @@ int gn_bwd(const void* dy, const void* x, const float* gamma, const float* beta,
   const T* xp = static_cast<const T*>(x);
   const T* gp = static_cast<const T*>(dy);
   T* op = static_cast<T*>(dx);
-  if (2 * batch * cut.S * (long)sizeof(T) > GN_CACHED)
+  if (2 * batch * cut.S * (long)sizeof(T) > GN_CACHED || cut.iters > GN_RUN)
     return cut_bwd<T, ACT, true>(gp, xp, gamma, beta, stats, op, dgamma, dbeta, part, batch, cut, dtype, s);
   return cut_bwd<T, ACT, false>(gp, xp, gamma, beta, stats, op, dgamma, dbeta, part, batch, cut, dtype, s);
 }

@@ -28,9 +28,9 @@ def orthogonalize(matrices: Union[torch.Tensor, Sequence[torch.Tensor]], steps: 
 
     ``X = u / max(|u|_F, eps)``, then ``steps`` times ``X <- (a I + b S + c S S) X`` with ``S = X X^T`` (on the transpose
     where rows exceed columns) and (a, b, c) = (3.4445, -4.775, 2.0315): singular values that are not tiny end between 0.7
-    and 1.2.  float32, bfloat16 or float16 in and out (one type per list), computed about as exactly as with
-    float32 products.  Returns new contiguous tensors; no gradient flows through.  A list may hold matrices of different sizes: tiles and splits are
-    chosen for all that share a launch, so a matrix's last bits can depend on its company.
+    and 1.2.  float32, bfloat16 or float16 in and out (one type per list), computed about as exactly as with float32
+    products.  Returns new contiguous tensors; no gradient flows through.  A list may hold matrices of different
+    sizes: tiles and splits are chosen for all that share a launch, so a matrix's last bits can depend on its company.
     """
     single = isinstance(matrices, torch.Tensor)
     ms = [matrices] if single else list(matrices)
