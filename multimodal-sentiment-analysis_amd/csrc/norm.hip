@@ -808,7 +808,8 @@ __global__ __launch_bounds__(1024) void gn_bwd_apply_kernel(const T* __restrict_
 // bundles of one sample run on one XCD, whose L2 they share.
 // One launch instead of three, one read instead of two.  256 x 512 x 128 bf16 in 16 groups, SiLU: 21 us, 67 MB at 3.2 TB/s
 // (chunks: 40 us); 32 x 2080 x 64 fp32 in 8 groups, ReLU: 15 us (22), backward 18.6 + 3.8 us (28); 1 x 128 x 256 in 32
-// groups: 4.7 us, which is the launch and two joins.  Bound by the wait for a block's own loads: its two sums cannot start before.
+// groups: 4.7 us, which is the launch and two joins.  Bound by the wait for a block's own loads: its two sums cannot
+// start before.
 struct Slab {
   long S;          // values per sample
   int P, C, G, Cg;
